@@ -32,6 +32,14 @@ enum {
   NTB200_DTYPE_I64 = 4
 };
 
+/* long-context scalings of the rotary frequencies (see ntb200_rope_cos_sin_cache) */
+enum {
+  NTB200_ROPE_NONE = 0,
+  NTB200_ROPE_LINEAR = 1,
+  NTB200_ROPE_NTK = 2,
+  NTB200_ROPE_YARN = 3
+};
+
 /* host-side status codes */
 enum {
   NTB200_OK = 0,
@@ -301,6 +309,104 @@ int ntb200_flash_attn_varlen(
     int64_t q_head_stride, int64_t k_token_stride, int64_t k_head_stride,
     int64_t v_token_stride, int64_t v_head_stride, int64_t out_token_stride,
     int64_t out_head_stride, int dtype, void* stream);
+
+/* ---------------------------------------------------------------------------------------
+ * Rotary embedding in either layout, in place, of the first rotary_dim dims of every
+ * query/key head: with c, s = cos_sin_cache[pos][i], cos_sin_cache[pos][rot/2 + i] a pair
+ * (a, b) becomes (a c - b s, b c + a s); the pair is dims (2i, 2i + 1) when interleaved != 0
+ * and (i, i + rot/2) otherwise.  fp32 arithmetic, one rounding of each result (unlike
+ * ntb200_rotary_embedding_neox, which rounds each product as vLLM's torch path does).  A part
+ * of a head that does not start at its first dim is a query/key pointer moved to it.
+ * cos_sin_cache [num_cache_rows, >= rotary_dim] of cache_dtype: F32, or the dtype of
+ * query/key.  key may be NULL.  dtype F32, BF16 or F16; positions I64 or I32.  Rows, strides
+ * and tables that are not 16-byte aligned run pair by pair; an interleaved pair must be
+ * aligned to its size (NTB200_ERR_MISALIGNED).  A token whose position is outside
+ * [0, num_cache_rows) is left untouched and sets NTB200_DEVERR_INDEX_RANGE.  Query and key
+ * must not overlap.  The reference rotates NeoX heads only
+ * (vllm_nt/_ntops/oot_support.py:134-204). */
+int ntb200_rotary_embedding(const void* positions, int positions_dtype, void* query, void* key,
+                            const void* cos_sin_cache, int cache_dtype, int64_t num_tokens,
+                            int64_t num_q_heads, int64_t num_k_heads, int64_t head_size,
+                            int64_t rotary_dim, int interleaved, int64_t q_token_stride,
+                            int64_t q_head_stride, int64_t k_token_stride, int64_t k_head_stride,
+                            int64_t cache_row_stride, int64_t num_cache_rows, int dtype,
+                            void* stream);
+
+/* The table those rotations read: row r of out [num_positions, >= rotary_dim] holds
+ * magnitude * cos(p f_i) in its first half and magnitude * sin(p f_i) in its second, with
+ * p = first_position + r and, for i < d/2 (d = rotary_dim), g_i = base^(-2i/d):
+ *   NTB200_ROPE_NONE    f_i = g_i
+ *   NTB200_ROPE_LINEAR  f_i = g_i / factor
+ *   NTB200_ROPE_NTK     g_i with base * factor^(d/(d-2)) for base
+ *   NTB200_ROPE_YARN    f_i = g_i / factor * w_i + g_i * (1 - w_i), w_i a ramp from 0 to 1 over
+ *                       i between the frequencies that make beta_fast and beta_slow turns over
+ *                       original_max_position positions (rounded outwards to whole i)
+ * each divided by freq_divisors[i] where given (fp32 [d/2], device memory).  The angle is
+ * formed and reduced to [-pi, pi] in fp64.  dtype F32, BF16 or F16; original_max_position,
+ * beta_fast and beta_slow are read for YARN only.  Replaces the host-side table of
+ * vLLM's RotaryEmbedding._compute_cos_sin_cache; the reference gathers from that one. */
+int ntb200_rope_cos_sin_cache(void* out, int64_t num_positions, int64_t first_position,
+                              int64_t rotary_dim, double base, int scaling, double factor,
+                              double original_max_position, double beta_fast, double beta_slow,
+                              double magnitude, const float* freq_divisors,
+                              int64_t out_row_stride, int dtype, void* stream);
+
+/* ---------------------------------------------------------------------------------------
+ * One latent-attention layer's rows into its paged cache, in one launch:
+ *   y[t] = latent[t] * rsqrt(mean(latent[t]^2) + eps) * norm_weight   (latent[t] if NULL)
+ *   key[t] and query[t, h] (rope_dim dims each) rotated in place as ntb200_rotary_embedding
+ *   cache[slot / block_size, slot % block_size] = [y[t] | rotated key[t]],
+ *     slot = slot_mapping[t], for t < num_store_tokens with slot >= 0
+ *   latent_out[t] = y[t] where latent_out is not NULL (it may be latent itself)
+ * latent [tokens, latent_dim], key [tokens, rope_dim] (usually columns of one projection),
+ * query [tokens, heads, rope_dim] (the rotary columns of the query heads; may be NULL).
+ * fp32 arithmetic, one rounding.  Negative slots and rows past num_store_tokens (vLLM's
+ * padding) are normalised and rotated but not stored; slots >= num_slots are skipped and set
+ * NTB200_DEVERR_INDEX_RANGE, as does a position outside the table (its rows stay unrotated).
+ * Slots must differ.  dtype BF16 or F16 (cache, latent, key and query); cos_sin_cache F32 or
+ * dtype; latent_dim a multiple of 8 up to 1024, rope_dim of 16 up to 256; pointers 16-byte
+ * aligned, strides multiples of 8.  No counterpart in the reference. */
+int ntb200_latent_rope_and_cache(
+    const void* positions, int positions_dtype, void* query, const void* latent, void* key,
+    const void* norm_weight, float eps, const void* cos_sin_cache, int cache_dtype, int interleaved,
+    void* kv_cache, void* latent_out, const void* slot_mapping, int slot_dtype, int64_t num_tokens,
+    int64_t num_store_tokens, int64_t num_heads, int64_t latent_dim, int64_t rope_dim,
+    int64_t q_token_stride, int64_t q_head_stride, int64_t latent_token_stride,
+    int64_t key_token_stride, int64_t latent_out_token_stride, int64_t cos_sin_row_stride,
+    int64_t num_cos_sin_rows, int64_t block_size, int64_t num_slots, int64_t cache_block_stride,
+    int64_t cache_page_stride, int dtype, void* stream);
+
+/* ---------------------------------------------------------------------------------------
+ * Latent attention over the paged cache (absorbed form): for query token t of sequence b and
+ * head h, over the cached rows j = [latent_j (512) | key_j (64)] it sees,
+ *   s_j = scale * (q_latent[t, h] . latent_j + q_rope[t, h] . key_j)
+ *   out[t, h] = sum_j softmax(s)_j latent_j,   lse[t, h] = ln sum_j exp(s_j)
+ * Sequence b's queries are rows query_start_loc[b] .. query_start_loc[b + 1]; without
+ * query_start_loc (NULL) every sequence has num_tokens / num_seqs of them (1: a decode batch).
+ * They are the last of its seq_lens[b] cached tokens: query i sees positions up to
+ * seq_lens[b] - q_len + i.  A row that sees nothing is zero, its lse -inf; rows behind the last
+ * sequence are left as they were.  fp32 softmax and accumulation, the weights rounded to the
+ * input type for their product.  lse may be NULL.
+ * Cache [num_blocks, block_size, 576], block_size a multiple of 16; block_tables int32
+ * [num_seqs, max_blocks_per_seq].  max_query_len bounds every query count (longer sequences are
+ * skipped), max_seq_len every length (<= 0: max_blocks_per_seq * block_size; it only sizes
+ * the launch).  Page ids out of range (their rows read as zeros), lengths beyond the block table
+ * (clamped) and inconsistent query_start_loc (skipped) set NTB200_DEVERR_INDEX_RANGE.
+ * latent_dim 512, rope_dim 64, dtype BF16 or F16, any number of heads; pointers 16-byte
+ * aligned, strides multiples of 8.  workspace: ntb200_latent_attention_workspace_size() bytes,
+ * 256-byte aligned, of the current device; two calls may share it only in stream order.
+ * No counterpart in the reference. */
+size_t ntb200_latent_attention_workspace_size(void);
+int ntb200_latent_attention(
+    void* out, float* lse, const void* q_latent, const void* q_rope, const void* kv_cache,
+    const int32_t* query_start_loc, const int32_t* seq_lens, const int32_t* block_tables,
+    int64_t num_seqs, int64_t num_tokens, int64_t num_heads, int64_t latent_dim, int64_t rope_dim,
+    int64_t block_size, int64_t num_blocks, int64_t max_blocks_per_seq, int64_t block_table_stride,
+    int64_t max_query_len, int64_t max_seq_len, float scale, int64_t ql_token_stride,
+    int64_t ql_head_stride, int64_t qr_token_stride, int64_t qr_head_stride,
+    int64_t out_token_stride, int64_t out_head_stride, int64_t lse_token_stride,
+    int64_t cache_block_stride, int64_t cache_page_stride, void* workspace, size_t workspace_bytes,
+    int dtype, void* stream);
 
 /* ---------------------------------------------------------------------------------------
  * Dense projection  out[M, N] = x[M, K] . weight[N, K]^T (+ bias[N]),  fp32 accumulate,

@@ -35,6 +35,9 @@ KERNEL_SOURCES = (
     "silu_and_mul.cu",
     "rope.cu",
     "rope_cache.cu",
+    "rotary.cu",
+    "latent_cache.cu",
+    "latent_attention.cu",
     "kv_cache.cu",
     "embedding.cu",
     "paged_decode.cu",
@@ -44,7 +47,8 @@ KERNEL_SOURCES = (
     "allreduce.cu",
     "sampler.cu",
 )
-SHARED_HEADERS = (CSRC / "common.cuh", CSRC / "tcgen05.cuh", CSRC / "rope_math.cuh", INCLUDE / "ntb200.h", Path(__file__).resolve())
+SHARED_HEADERS = (CSRC / "common.cuh", CSRC / "tcgen05.cuh", CSRC / "rope_math.cuh", CSRC / "rope_layout.cuh",
+                  INCLUDE / "ntb200.h", Path(__file__).resolve())
 
 NVCC_FLAGS = [
     "-gencode",

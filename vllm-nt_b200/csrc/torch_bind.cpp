@@ -722,6 +722,205 @@ void random_sample(at::Tensor out, const at::Tensor& probs, const at::Tensor& q)
                              probs.size(1), probs.stride(0), q.stride(0), stream_of(probs)),
         "random_sample");
 }
+void same_device(const at::Tensor& a, const at::Tensor& b, const char* what) {
+  TORCH_CHECK(b.is_cuda() && a.device() == b.device(), "ntb200.", what, ": tensors on different devices");
+}
+
+int index_code(const at::Tensor& t, const char* what, const char* name) {
+  TORCH_CHECK(t.scalar_type() == at::kInt || t.scalar_type() == at::kLong, "ntb200.", what, ": ", name,
+              " must be int32 or int64");
+  return dtype_code(t);
+}
+
+// Rotation in either layout, in place, with an fp32 table or one of query's dtype.
+void rotary_embedding(const at::Tensor& positions, at::Tensor query, const std::optional<at::Tensor>& key,
+                      const at::Tensor& cache, int64_t head_size, int64_t rotary_dim, bool interleaved) {
+  require_cuda(query, "query");
+  require_rows(cache, "cos_sin_cache");
+  same_device(query, positions, "rotary_embedding");
+  same_device(query, cache, "rotary_embedding");
+  TORCH_CHECK(positions.is_contiguous(), "ntb200.rotary_embedding: positions must be contiguous");
+  TORCH_CHECK(cache.scalar_type() == query.scalar_type() || cache.scalar_type() == at::kFloat,
+              "ntb200.rotary_embedding: cos_sin_cache must be float32 or of query's dtype");
+  TORCH_CHECK(rotary_dim <= cache.size(1), "ntb200.rotary_embedding: rotary_dim exceeds cos_sin_cache's rows");
+  TORCH_CHECK(head_size > 0, "ntb200.rotary_embedding: head_size must be positive");
+  const int64_t tokens = positions.numel();
+  int64_t hq = 0, qts = 0, qhs = 0, hk = 0, kts = 0, khs = 0;
+  head_geometry(query, tokens, head_size, "query", hq, qts, qhs);
+  void* kptr = nullptr;
+  if (key.has_value()) {
+    same_device(query, *key, "rotary_embedding");
+    TORCH_CHECK(key->scalar_type() == query.scalar_type(), "ntb200.rotary_embedding: key dtype must match query");
+    head_geometry(*key, tokens, head_size, "key", hk, kts, khs);
+    kptr = key->data_ptr();
+  }
+  c10::cuda::CUDAGuard guard(query.device());
+  check(ntb200_rotary_embedding(positions.data_ptr(), index_code(positions, "rotary_embedding", "positions"),
+                                query.data_ptr(), kptr, cache.data_ptr(), dtype_code(cache), tokens, hq, hk, head_size,
+                                rotary_dim, interleaved ? 1 : 0, qts, qhs, kts, khs,
+                                cache.size(0) > 1 ? cache.stride(0) : cache.size(1), cache.size(0), dtype_code(query),
+                                stream_of(query)),
+        "rotary_embedding");
+}
+
+// out [positions, >= rotary_dim] = cos | sin of the scaled frequencies
+void rope_cos_sin_cache(at::Tensor out, int64_t first_position, int64_t rotary_dim, double base, int64_t scaling,
+                        double factor, double original_max_position, double beta_fast, double beta_slow,
+                        double magnitude, const std::optional<at::Tensor>& freq_divisors) {
+  require_rows(out, "out");
+  TORCH_CHECK(rotary_dim > 0 && rotary_dim <= out.size(1), "ntb200.rope_cos_sin_cache: rotary_dim exceeds out's rows");
+  const float* div = nullptr;
+  if (freq_divisors.has_value()) {
+    same_device(out, *freq_divisors, "rope_cos_sin_cache");
+    TORCH_CHECK(freq_divisors->scalar_type() == at::kFloat && freq_divisors->is_contiguous() &&
+                    freq_divisors->numel() == rotary_dim / 2,
+                "ntb200.rope_cos_sin_cache: freq_divisors must be contiguous float32 [rotary_dim / 2]");
+    div = freq_divisors->data_ptr<float>();
+  }
+  c10::cuda::CUDAGuard guard(out.device());
+  check(ntb200_rope_cos_sin_cache(out.data_ptr(), out.size(0), first_position, rotary_dim, base,
+                                  static_cast<int>(scaling), factor, original_max_position, beta_fast, beta_slow,
+                                  magnitude, div, out.size(0) > 1 ? out.stride(0) : out.size(1), dtype_code(out),
+                                  stream_of(out)),
+        "rope_cos_sin_cache");
+}
+
+// Norm of the latent rows, rotation of the shared key and the queries, store into the latent
+// cache [blocks, block_size, latent_dim + rope_dim].
+void latent_rope_and_cache(const at::Tensor& positions, const std::optional<at::Tensor>& query,
+                           const at::Tensor& latent, at::Tensor key, const std::optional<at::Tensor>& norm_weight,
+                           double eps, const at::Tensor& cos_sin_cache, bool interleaved, at::Tensor kv_cache,
+                           const std::optional<at::Tensor>& latent_out, const at::Tensor& slot_mapping) {
+  const char* op = "latent_rope_and_cache";
+  require_rows(latent, "latent");
+  require_rows(key, "key");
+  require_rows(cos_sin_cache, "cos_sin_cache");
+  same_device(latent, key, op);
+  same_device(latent, positions, op);
+  same_device(latent, cos_sin_cache, op);
+  same_device(latent, kv_cache, op);
+  same_device(latent, slot_mapping, op);
+  const int64_t tokens = latent.size(0), ld = latent.size(1), rd = key.size(1);
+  const auto dt = latent.scalar_type();
+  TORCH_CHECK(positions.is_contiguous() && positions.numel() == tokens && key.size(0) == tokens,
+              "ntb200.latent_rope_and_cache: positions [tokens] contiguous, key [tokens, rope_dim]");
+  TORCH_CHECK(slot_mapping.dim() == 1 && slot_mapping.is_contiguous() && slot_mapping.size(0) <= tokens,
+              "ntb200.latent_rope_and_cache: slot_mapping must be 1-D contiguous, <= tokens");
+  TORCH_CHECK(kv_cache.dim() == 3 && kv_cache.size(2) == ld + rd && kv_cache.stride(2) == 1 && kv_cache.size(1) > 0,
+              "ntb200.latent_rope_and_cache: kv_cache must be [blocks, block_size, latent_dim + rope_dim]");
+  TORCH_CHECK(key.scalar_type() == dt && kv_cache.scalar_type() == dt &&
+                  (cos_sin_cache.scalar_type() == dt || cos_sin_cache.scalar_type() == at::kFloat),
+              "ntb200.latent_rope_and_cache: latent, key and kv_cache of one dtype, cos_sin_cache of it or float32");
+  TORCH_CHECK(cos_sin_cache.size(1) >= rd, "ntb200.latent_rope_and_cache: cos_sin_cache rows shorter than the key");
+  int64_t hq = 0, qts = 0, qhs = 0, los = 0;
+  void* q = nullptr;
+  if (query.has_value()) {
+    same_device(latent, *query, op);
+    TORCH_CHECK(query->scalar_type() == dt && query->dim() == 3, "ntb200.latent_rope_and_cache: query must be "
+                "[tokens, heads, rope_dim] of latent's dtype");
+    head_geometry(*query, tokens, rd, "query", hq, qts, qhs);
+    q = query->data_ptr();
+  }
+  const void* w = nullptr;
+  if (norm_weight.has_value()) same_device(latent, *norm_weight, op), w = ::norm_weight(norm_weight, latent, ld, op);
+  void* lo = nullptr;
+  if (latent_out.has_value()) {
+    require_rows(*latent_out, "latent_out");
+    same_device(latent, *latent_out, op);
+    TORCH_CHECK(latent_out->sizes() == latent.sizes() && latent_out->scalar_type() == dt,
+                "ntb200.latent_rope_and_cache: latent_out must be like latent");
+    lo = latent_out->data_ptr();
+    los = tokens > 1 ? latent_out->stride(0) : ld;
+  }
+  c10::cuda::CUDAGuard guard(latent.device());
+  check(ntb200_latent_rope_and_cache(
+            positions.data_ptr(), index_code(positions, op, "positions"), q, latent.data_ptr(), key.data_ptr(), w,
+            static_cast<float>(eps), cos_sin_cache.data_ptr(), dtype_code(cos_sin_cache), interleaved ? 1 : 0,
+            kv_cache.data_ptr(), lo, slot_mapping.data_ptr(), index_code(slot_mapping, op, "slot_mapping"), tokens,
+            slot_mapping.size(0), hq, ld, rd, tokens > 1 ? qts : 0, hq > 1 ? qhs : 0, tokens > 1 ? latent.stride(0) : 0,
+            tokens > 1 ? key.stride(0) : 0, los, cos_sin_cache.size(0) > 1 ? cos_sin_cache.stride(0) : cos_sin_cache.size(1),
+            cos_sin_cache.size(0), kv_cache.size(1), kv_cache.size(0) * kv_cache.size(1),
+            kv_cache.size(0) > 1 ? kv_cache.stride(0) : 0, kv_cache.size(1) > 1 ? kv_cache.stride(1) : ld + rd,
+            dtype_code(latent), stream_of(latent)),
+        op);
+}
+
+int64_t latent_attention_workspace_size() { return static_cast<int64_t>(ntb200_latent_attention_workspace_size()); }
+
+// Absorbed latent attention over the paged cache; query_start_loc absent: the same number of
+// queries for every sequence.
+void latent_attention(at::Tensor out, const std::optional<at::Tensor>& lse, const at::Tensor& q_latent,
+                      const at::Tensor& q_rope, const at::Tensor& kv_cache,
+                      const std::optional<at::Tensor>& query_start_loc, const at::Tensor& seq_lens,
+                      const at::Tensor& block_table, int64_t max_query_len, int64_t max_seq_len, double scale,
+                      const std::optional<at::Tensor>& workspace) {
+  const char* op = "latent_attention";
+  require_cuda(q_latent, "q_latent");
+  same_device(q_latent, out, op);
+  same_device(q_latent, q_rope, op);
+  same_device(q_latent, kv_cache, op);
+  same_device(q_latent, seq_lens, op);
+  same_device(q_latent, block_table, op);
+  const auto dt = q_latent.scalar_type();
+  TORCH_CHECK(q_latent.dim() == 3 && q_rope.dim() == 3 && q_latent.stride(2) == 1 && q_rope.stride(2) == 1 &&
+                  q_rope.size(0) == q_latent.size(0) && q_rope.size(1) == q_latent.size(1) &&
+                  q_rope.scalar_type() == dt,
+              "ntb200.latent_attention: q_latent [tokens, heads, latent_dim], q_rope [tokens, heads, rope_dim]");
+  TORCH_CHECK(out.sizes() == q_latent.sizes() && out.stride(2) == 1 && out.scalar_type() == dt,
+              "ntb200.latent_attention: out must be like q_latent");
+  TORCH_CHECK(kv_cache.dim() == 3 && kv_cache.size(2) == q_latent.size(2) + q_rope.size(2) && kv_cache.stride(2) == 1 &&
+                  kv_cache.scalar_type() == dt,
+              "ntb200.latent_attention: kv_cache must be [blocks, block_size, latent_dim + rope_dim] like q_latent");
+  const int64_t tokens = q_latent.size(0), heads = q_latent.size(1), blocks = kv_cache.size(0), bs = kv_cache.size(1);
+  TORCH_CHECK(seq_lens.scalar_type() == at::kInt && seq_lens.is_contiguous() && seq_lens.dim() == 1 &&
+                  block_table.scalar_type() == at::kInt && block_table.dim() == 2 &&
+                  (block_table.size(1) <= 1 || block_table.stride(1) == 1),
+              "ntb200.latent_attention: seq_lens int32 [seqs], block_table int32 [seqs, max_blocks]");
+  int64_t seqs = seq_lens.size(0);
+  const int32_t* qsl = nullptr;
+  if (query_start_loc.has_value()) {
+    same_device(q_latent, *query_start_loc, op);
+    TORCH_CHECK(query_start_loc->scalar_type() == at::kInt && query_start_loc->is_contiguous() &&
+                    query_start_loc->dim() == 1 && query_start_loc->numel() >= 1 &&
+                    query_start_loc->numel() - 1 <= seqs,
+                "ntb200.latent_attention: query_start_loc must be int32 contiguous [seqs + 1]");
+    seqs = query_start_loc->numel() - 1;
+    qsl = query_start_loc->data_ptr<int32_t>();
+  }
+  TORCH_CHECK(block_table.size(0) >= seqs, "ntb200.latent_attention: block_table has fewer rows than sequences");
+  float* l = nullptr;
+  int64_t ls = 0;
+  if (lse.has_value()) {
+    same_device(q_latent, *lse, op);
+    TORCH_CHECK(lse->scalar_type() == at::kFloat && lse->dim() == 2 && lse->size(0) == tokens && lse->size(1) == heads &&
+                    (heads == 1 || lse->stride(1) == 1),
+                "ntb200.latent_attention: lse must be float32 [tokens, heads]");
+    l = lse->data_ptr<float>();
+    ls = lse->stride(0);
+  }
+  c10::cuda::CUDAGuard guard(q_latent.device());
+  const size_t need = ntb200_latent_attention_workspace_size();
+  at::Tensor ws;
+  if (workspace.has_value()) {
+    ws = *workspace;
+    same_device(q_latent, ws, op);
+    TORCH_CHECK(ws.is_contiguous(), "ntb200.latent_attention: workspace must be contiguous");
+  } else {
+    ws = at::empty({static_cast<int64_t>(need)}, q_latent.options().dtype(at::kByte));
+  }
+  const bool one = tokens <= 1, lone = heads <= 1;
+  check(ntb200_latent_attention(
+            out.data_ptr(), l, q_latent.data_ptr(), q_rope.data_ptr(), kv_cache.data_ptr(), qsl,
+            seq_lens.data_ptr<int32_t>(), block_table.data_ptr<int32_t>(), seqs, tokens, heads, q_latent.size(2),
+            q_rope.size(2), bs, blocks, block_table.size(1),
+            block_table.size(0) > 1 ? block_table.stride(0) : block_table.size(1), max_query_len, max_seq_len,
+            static_cast<float>(scale), one ? 0 : q_latent.stride(0), lone ? 0 : q_latent.stride(1),
+            one ? 0 : q_rope.stride(0), lone ? 0 : q_rope.stride(1), one ? 0 : out.stride(0), lone ? 0 : out.stride(1),
+            ls, blocks > 1 ? kv_cache.stride(0) : 0, bs > 1 ? kv_cache.stride(1) : kv_cache.size(2), ws.data_ptr(),
+            static_cast<size_t>(ws.numel() * ws.element_size()), dtype_code(q_latent), stream_of(q_latent)),
+        op);
+}
+
 }  // namespace
 
 TORCH_LIBRARY(ntb200, m) {
@@ -792,6 +991,21 @@ TORCH_LIBRARY(ntb200, m) {
   m.def("allreduce_buffer_size(int capacity, int elem_bytes, int world_size) -> int", &allreduce_buffer_size);
   m.def("top_k_top_p(Tensor(a!) logits, Tensor? k, Tensor? p) -> ()");
   m.def("random_sample(Tensor(a!) out, Tensor probs, Tensor q) -> ()");
+  m.def(
+      "rotary_embedding(Tensor positions, Tensor(a!) query, Tensor(b!)? key, Tensor cos_sin_cache, int head_size, "
+      "int rotary_dim, bool interleaved) -> ()");
+  m.def(
+      "rope_cos_sin_cache(Tensor(a!) out, int first_position, int rotary_dim, float base, int scaling, float factor, "
+      "float original_max_position, float beta_fast, float beta_slow, float magnitude, Tensor? freq_divisors) -> ()");
+  m.def(
+      "latent_rope_and_cache(Tensor positions, Tensor(a!)? query, Tensor latent, Tensor(b!) key, "
+      "Tensor? norm_weight, float eps, Tensor cos_sin_cache, bool interleaved, Tensor(c!) kv_cache, "
+      "Tensor(d!)? latent_out, Tensor slot_mapping) -> ()");
+  m.def("latent_attention_workspace_size() -> int", &latent_attention_workspace_size);
+  m.def(
+      "latent_attention(Tensor(a!) out, Tensor(b!)? lse, Tensor q_latent, Tensor q_rope, Tensor kv_cache, "
+      "Tensor? query_start_loc, Tensor seq_lens, Tensor block_table, int max_query_len, int max_seq_len, "
+      "float scale, Tensor(c!)? workspace) -> ()");
 }
 
 TORCH_LIBRARY_IMPL(ntb200, CUDA, m) {
@@ -820,4 +1034,8 @@ TORCH_LIBRARY_IMPL(ntb200, CUDA, m) {
   m.impl("attention_flash_layout", &attention_flash_layout);
   m.impl("top_k_top_p", &top_k_top_p);
   m.impl("random_sample", &random_sample);
+  m.impl("rotary_embedding", &rotary_embedding);
+  m.impl("rope_cos_sin_cache", &rope_cos_sin_cache);
+  m.impl("latent_rope_and_cache", &latent_rope_and_cache);
+  m.impl("latent_attention", &latent_attention);
 }

@@ -8,12 +8,13 @@ for a non-zero status."""
 from __future__ import annotations
 
 import ctypes
-from ctypes import c_char_p, c_float, c_int, c_int64, c_size_t, c_void_p
+from ctypes import c_char_p, c_double, c_float, c_int, c_int64, c_size_t, c_void_p
 from pathlib import Path
 
 LIBRARY = Path(__file__).resolve().parents[1] / "_lib" / "libntb200.so"
 
 DTYPE_F32, DTYPE_BF16, DTYPE_F16, DTYPE_I32, DTYPE_I64 = 0, 1, 2, 3, 4
+ROPE_NONE, ROPE_LINEAR, ROPE_NTK, ROPE_YARN = 0, 1, 2, 3
 DEVERR_WAIT_TIMEOUT, DEVERR_INDEX_RANGE = 1, 2
 
 # name -> (restype, argtypes); mirrors include/ntb200.h
@@ -94,6 +95,25 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
         [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_int64,
          c_int64, c_int64, c_int64, c_int64, c_int64, c_int64, c_float, c_int64, c_int64,
          c_int64, c_int64, c_int64, c_int64, c_int64, c_int, c_void_p],
+    ),
+    "ntb200_rotary_embedding": (
+        c_int,
+        [c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_int] + [c_int64] * 5 + [c_int] + [c_int64] * 6
+        + [c_int, c_void_p],
+    ),
+    "ntb200_rope_cos_sin_cache": (
+        c_int,
+        [c_void_p, c_int64, c_int64, c_int64, c_double, c_int] + [c_double] * 5 + [c_void_p, c_int64, c_int, c_void_p],
+    ),
+    "ntb200_latent_rope_and_cache": (
+        c_int,
+        [c_void_p, c_int] + [c_void_p] * 4 + [c_float, c_void_p, c_int, c_int] + [c_void_p] * 3 + [c_int]
+        + [c_int64] * 16 + [c_int, c_void_p],
+    ),
+    "ntb200_latent_attention_workspace_size": (c_size_t, []),
+    "ntb200_latent_attention": (
+        c_int,
+        [c_void_p] * 8 + [c_int64] * 11 + [c_float] + [c_int64] * 9 + [c_void_p, c_size_t, c_int, c_void_p],
     ),
     "ntb200_linear_workspace_size": (c_size_t, [c_int64, c_int64, c_int64]),
     "ntb200_linear": (

@@ -49,6 +49,10 @@ def _register_fakes() -> None:
         "attention_flash_layout",
         "top_k_top_p",
         "random_sample",
+        "rotary_embedding",
+        "rope_cos_sin_cache",
+        "latent_rope_and_cache",
+        "latent_attention",
     ):
         torch.library.register_fake(f"ntb200::{name}")(nothing)
 

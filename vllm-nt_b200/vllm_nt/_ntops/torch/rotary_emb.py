@@ -1,12 +1,19 @@
-"""In-place NeoX rotary embedding on the sm_100a kernel (replaces
+"""In-place rotary embedding on the sm_100a kernels (replaces
 vllm_nt/_ntops/torch/rotary_emb.py and the cos/sin gather of
-vllm_nt/_ntops/oot_support.py:164-204)."""
+vllm_nt/_ntops/oot_support.py:164-204): NeoX heads with a table of their own dtype as vLLM
+rounds them, the interleaved layout and fp32 tables with one rounding, and the table itself."""
 
 from __future__ import annotations
 
+import math
+
 import torch
 
+from vllm_nt._ntops import capi
 from vllm_nt._ntops.torch._ext import ops
+
+_SCALINGS = {None: capi.ROPE_NONE, "none": capi.ROPE_NONE, "linear": capi.ROPE_LINEAR, "ntk": capi.ROPE_NTK,
+             "yarn": capi.ROPE_YARN}
 
 
 def _heads(t: torch.Tensor, num_tokens: int, head_size: int) -> torch.Tensor:
@@ -23,11 +30,17 @@ def rotary_embedding(
     head_size: int,
     cos_sin_cache: torch.Tensor,
     rotary_dim: int | None = None,
+    interleaved: bool = False,
 ) -> tuple[torch.Tensor, torch.Tensor | None]:
-    """Rotates the first ``rotary_dim`` dims of every head of query (and key) in place,
-    NeoX style, with cos/sin = cos_sin_cache[positions] split in halves.  The cache must
-    already have query's dtype (vLLM's _match_cos_sin_cache_dtype)."""
+    """Rotates the first ``rotary_dim`` dims of every head of query (and key) in place, with
+    cos/sin = cos_sin_cache[positions] split in halves.  Pairs are (i, i + rotary_dim / 2)
+    (NeoX), or (2i, 2i + 1) with ``interleaved``.  NeoX pairs and a cache of query's dtype
+    (vLLM's _match_cos_sin_cache_dtype) are rounded as vLLM's torch path rounds them; an fp32
+    cache of 16-bit heads, and interleaved pairs, are rotated in fp32 and rounded once.  Heads
+    that are a column slice (the rotary part at a head's end) are passed as the 3-D slice."""
     rot = cos_sin_cache.shape[-1] if rotary_dim is None else rotary_dim
+    if interleaved or cos_sin_cache.dtype != query.dtype:
+        return _rotary_either_layout(positions, query, key, int(head_size), cos_sin_cache, int(rot), bool(interleaved))
     if (positions.is_contiguous() and cos_sin_cache.is_contiguous() and query.dim() == 2
             and query.stride(-1) == 1 and (key is None or (key.dim() == 2 and key.stride(-1) == 1))):
         # vLLM's [tokens, heads * head_size] slices of the qkv projection go straight in
@@ -42,6 +55,66 @@ def rotary_embedding(
     k = _heads(key, n, head_size) if key is not None else None
     ops().rotary_embedding_neox(positions, q, k, cache, int(head_size), int(rot))
     return query, key
+
+
+def _sliced_heads(t: torch.Tensor, num_tokens: int, head_size: int) -> torch.Tensor:
+    """[tokens, heads, head_size] of rows of heads, or of a 3-D slice as it is."""
+    if t.dim() == 3 and t.shape[0] == num_tokens and t.shape[2] == head_size and t.stride(2) == 1:
+        return t
+    return _heads(t, num_tokens, head_size)
+
+
+def _rotary_either_layout(positions, query, key, head_size, cos_sin_cache, rot, interleaved):
+    positions = positions.reshape(-1)
+    if not positions.is_contiguous():
+        positions = positions.contiguous()
+    n = positions.shape[0]
+    cache = cos_sin_cache if cos_sin_cache.stride(-1) == 1 else cos_sin_cache.contiguous()
+    q = _sliced_heads(query, n, head_size)
+    k = _sliced_heads(key, n, head_size) if key is not None else None
+    ops().rotary_embedding(positions, q, k, cache, head_size, rot, interleaved)
+    return query, key
+
+
+def rope_cos_sin_cache(
+    num_positions: int,
+    rotary_dim: int,
+    base: float = 10000.0,
+    *,
+    scaling: str | None = None,
+    factor: float = 1.0,
+    original_max_position: int | None = None,
+    beta_fast: float = 32.0,
+    beta_slow: float = 1.0,
+    magnitude: float | None = None,
+    freq_divisors: torch.Tensor | None = None,
+    first_position: int = 0,
+    dtype: torch.dtype = torch.float32,
+    device: torch.device | str | None = None,
+    out: torch.Tensor | None = None,
+) -> torch.Tensor:
+    """The [num_positions, rotary_dim] table cat(cos, sin) of position * frequency that the
+    rotary kernels read, angles formed in 64 bits.  ``scaling`` stretches the frequencies
+    base^(-2i/d) to contexts ``factor`` times as long: ``"linear"`` divides them by factor,
+    ``"ntk"`` raises base to base * factor^(d/(d-2)), ``"yarn"`` divides those that turn less
+    than ``beta_slow`` times over ``original_max_position`` positions, keeps those that turn more
+    than ``beta_fast`` times and blends between.  ``freq_divisors`` (float32 [d/2]) divide the
+    frequencies one by one.  cos and sin are multiplied by ``magnitude`` (None: 0.1 ln(factor) + 1
+    for yarn with factor > 1, else 1).  ``out`` may be given instead of dtype and device."""
+    if scaling not in _SCALINGS:
+        raise ValueError(f"rope_cos_sin_cache: unknown scaling {scaling!r}")
+    if scaling == "yarn" and original_max_position is None:
+        raise ValueError("rope_cos_sin_cache: yarn needs original_max_position")
+    if magnitude is None:
+        magnitude = 0.1 * math.log(factor) + 1.0 if scaling == "yarn" and factor > 1.0 else 1.0
+    if out is None:
+        out = torch.empty(num_positions, rotary_dim, dtype=dtype, device="cuda" if device is None else device)
+    elif out.dim() != 2 or out.shape[0] != num_positions:
+        raise ValueError("rope_cos_sin_cache: out must be [num_positions, >= rotary_dim]")
+    ops().rope_cos_sin_cache(out, int(first_position), int(rotary_dim), float(base), _SCALINGS[scaling], float(factor),
+                             float(original_max_position or 0), float(beta_fast), float(beta_slow), float(magnitude),
+                             freq_divisors)
+    return out
 
 
 def rotary_embedding_and_cache(
