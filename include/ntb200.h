@@ -409,6 +409,31 @@ int ntb200_latent_attention(
     int dtype, void* stream);
 
 /* ---------------------------------------------------------------------------------------
+ * Latent attention over keys and values expanded from the latent (prompts): per head h
+ *   s_ij = scale * (query[i, h] . [k_nope[j, h] | k_rope[j]]),
+ *   out[i, h] = sum_j softmax(s_i)_j value[j, h],   lse[i, h] = ln sum_j exp(s_ij)
+ * query [num_q_tokens, heads, 192] (nope 128, then rope 64), k_nope and value
+ * [num_k_tokens, heads, 128] (usually halves of one up-projection's rows), k_rope
+ * [num_k_tokens, 64], the rotary key that all heads share.  Sequences and causal masking as
+ * ntb200_flash_attn_varlen: queries at rows cu_seqlens_q[b] .. cu_seqlens_q[b + 1], keys at
+ * rows cu_seqlens_k[b] .. cu_seqlens_k[b + 1], aligned to the end of the keys.  fp32 softmax
+ * and accumulation, the weights rounded to the input type.  A row that sees no key is zero, its
+ * lse -inf; rows behind the last sequence are left as they were; lse may be NULL.
+ * max_query_len bounds the query counts (it only sizes the launch).  Sequences that reach
+ * outside num_q_tokens or num_k_tokens are skipped and set NTB200_DEVERR_INDEX_RANGE.
+ * dtype BF16 or F16, scale > 0; pointers 16-byte aligned, strides multiples of 8.
+ * No workspace.  No counterpart in the reference. */
+int ntb200_latent_attention_prefill(
+    void* out, float* lse, const void* query, const void* k_nope, const void* k_rope,
+    const void* value, const int32_t* cu_seqlens_q, const int32_t* cu_seqlens_k, int64_t num_seqs,
+    int64_t num_q_tokens, int64_t num_k_tokens, int64_t num_heads, int64_t nope_dim,
+    int64_t rope_dim, int64_t v_dim, int64_t max_query_len, float scale, int causal,
+    int64_t q_token_stride, int64_t q_head_stride, int64_t kn_token_stride, int64_t kn_head_stride,
+    int64_t kr_token_stride, int64_t v_token_stride, int64_t v_head_stride,
+    int64_t out_token_stride, int64_t out_head_stride, int64_t lse_token_stride, int dtype,
+    void* stream);
+
+/* ---------------------------------------------------------------------------------------
  * Dense projection  out[M, N] = x[M, K] . weight[N, K]^T (+ bias[N]),  fp32 accumulate,
  * tcgen05/TMEM tensor cores fed by TMA.  dtype BF16 or F16; K a multiple of 8, rows 16-byte
  * aligned.  bias may be NULL.

@@ -13,7 +13,7 @@ import torch
 
 from _util import cuda_device, seeded, stream
 from vllm_nt._ntops import capi
-from vllm_nt._ntops.torch import latent_attention, latent_rope_and_cache, latent_workspace_bytes
+from vllm_nt._ntops.torch import latent_attention, latent_attention_prefill
 
 pytestmark = pytest.mark.gpu
 
@@ -181,3 +181,106 @@ def test_many_short_sequences_share_a_cta(heads):
     g = seeded(3)
     lens = torch.randint(1, 200, (700,), generator=g).tolist()
     check_attention(lens, [1] * 700, heads, 16, torch.bfloat16, 11)
+
+
+# ---- the expanded form ----
+
+
+def reference_expanded(q, kn, kr, v, qs, ks, causal):
+    """out, lse and their tolerances in 64 bits (the bounds of `reference`, 192 products a score)."""
+    u = U[q.dtype]
+    t, h, _ = q.shape
+    out, lse, tol = torch.zeros(t, h, 128).double(), torch.zeros(t, h).double(), torch.zeros(t, h, 128).double()
+    lse_tol = torch.zeros(t, h).double()
+    for b in range(len(qs) - 1):
+        q0, q1, k0, k1 = qs[b], qs[b + 1], ks[b], ks[b + 1]
+        nq, nk = q1 - q0, k1 - k0
+        for j in range(h):
+            qq = q[q0:q1, j].double()
+            kk = torch.cat((kn[k0:k1, j], kr[k0:k1]), -1).double()
+            vv = v[k0:k1, j].double()
+            s = qq @ kk.T * SCALE
+            hidden = torch.ones(nq, nk, dtype=torch.bool).triu(nk - nq + 1) if causal else torch.zeros(nq, nk, dtype=torch.bool)
+            s = s.masked_fill(hidden, -torch.inf)
+            ds = 192 * 2.0**-24 * SCALE * (qq.abs() @ kk.abs().T).amax(-1) if nk else torch.zeros(nq).double()
+            lse[q0:q1, j] = torch.logsumexp(s, -1)
+            w = torch.nan_to_num(torch.softmax(s, -1))
+            mag = w @ vv.abs()
+            out[q0:q1, j] = w @ vv
+            tol[q0:q1, j] = u * (mag + out[q0:q1, j].abs()) + (2 * ds[:, None] + 2.0**-20) * mag
+            if q.dtype == torch.float16 and nk:
+                tol[q0:q1, j] += nk * 2.0**-32 * vv.abs().max() + 2.0**-25
+            lse_tol[q0:q1, j] = ds + (nk + 64) * 2.0**-24 + 2.0**-21 * lse[q0:q1, j].abs()
+    return out, lse, tol, lse_tol
+
+
+def check_expanded(q_lens, k_lens, heads, dtype, seed, *, causal=True, tail=3, separate=False, use_lse=True, q_scale=1.0):
+    dev = cuda_device()
+    g = seeded(seed)
+    qs, ks = [0], [0]
+    for a, b in zip(q_lens, k_lens):
+        qs.append(qs[-1] + a)
+        ks.append(ks[-1] + b)
+    t, n, k = qs[-1] + tail, qs[-1], ks[-1] + tail
+    q = (torch.randn(t, heads, 192, generator=g) * q_scale).to(dtype)
+    kv = torch.randn(k, heads, 256, generator=g).to(dtype)
+    kr = torch.randn(k, 64, generator=g).to(dtype)
+    kv[ks[-1] :], kr[ks[-1] :], q[n:] = float("nan"), float("nan"), float("nan")  # rows behind the last sequence
+    kvd, qd, krd = kv.to(dev), q.to(dev), kr.to(dev)
+    knd, vd = kvd[..., :128], kvd[..., 128:]
+    if separate:
+        knd, vd = knd.contiguous(), vd.contiguous()
+    out = torch.full((t, heads, 128), 7.0, dtype=dtype, device=dev)
+    lse = torch.full((t, heads), 7.0, device=dev) if use_lse else None
+    latent_attention_prefill(out, qd, knd, krd, vd, torch.tensor(qs, dtype=torch.int32, device=dev),
+                             torch.tensor(ks, dtype=torch.int32, device=dev), max(q_lens), SCALE, causal, lse)
+    torch.cuda.synchronize()
+    assert capi.read_device_error(stream()) == 0
+    ref, ref_lse, tol, lse_tol = reference_expanded(q[:n], kv[..., :128], kr, kv[..., 128:], qs, ks, causal)
+    got = out.cpu().double()
+    assert bool((got[n:] == 7.0).all())
+    err = (got[:n] - ref).abs()
+    assert bool((err <= tol).all()), (err - tol).max()
+    if use_lse:
+        got_lse = lse.cpu().double()
+        assert bool((got_lse[n:] == 7.0).all())
+        empty = ref_lse == -torch.inf
+        assert torch.equal(got_lse[:n] == -torch.inf, empty)
+        e = (got_lse[:n] - ref_lse).abs()[~empty]
+        assert bool((e <= lse_tol[~empty]).all()), (e - lse_tol[~empty]).max()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("causal", [True, False])
+def test_expanded_at_tile_edges(causal, dtype):
+    """Prompts that end at, before and after a 16-step, a 128-row tile and a 256-row item; the next
+    sequence's rows follow directly."""
+    lens = [1, 15, 16, 17, 127, 128, 129, 255, 256, 257, 400, 0, 2]
+    check_expanded(lens, lens, 3, dtype, 21, causal=causal)
+
+
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("q_lens,k_lens", [([1, 1, 3], [500, 1, 129]), ([130, 20], [700, 300]), ([300, 5, 64], [100, 0, 64])])
+def test_expanded_queries_at_the_end_of_longer_or_shorter_contexts(q_lens, k_lens, causal):
+    """Cached prefixes, no keys at all, and more queries than keys (causal: rows that see nothing)."""
+    check_expanded(q_lens, k_lens, 5, torch.bfloat16, 22, causal=causal)
+
+
+@pytest.mark.parametrize("heads", [1, 10, 128])
+def test_expanded_heads_and_separate_tensors(heads):
+    check_expanded([70, 200], [70, 260], heads, torch.float16, heads, separate=True, use_lse=heads != 10)
+
+
+def test_expanded_long_prompt():
+    check_expanded([2100], [2100], 2, torch.bfloat16, 23)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_expanded_peaked_scores(dtype):
+    check_expanded([300, 40], [300, 900], 2, dtype, 24, q_scale=40.0)
+
+
+def test_expanded_many_short_prompts():
+    g = seeded(25)
+    lens = torch.randint(0, 40, (150,), generator=g).tolist()
+    check_expanded(lens, lens, 3, torch.bfloat16, 26)

@@ -38,6 +38,7 @@ KERNEL_SOURCES = (
     "rotary.cu",
     "latent_cache.cu",
     "latent_attention.cu",
+    "latent_prefill.cu",
     "kv_cache.cu",
     "embedding.cu",
     "paged_decode.cu",

@@ -248,4 +248,10 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, unsign
   }
 }
 
+// The same wait made by a whole warp, with one answer for all of it: a lane that gave up takes the
+// others along, so that none is left waiting for it in a warp-wide instruction.
+__device__ __forceinline__ bool mbar_wait_warp(uint64_t* bar, uint32_t parity, unsigned int* err) {
+  return __all_sync(0xffffffffu, mbar_wait(bar, parity, err));
+}
+
 }  // namespace ntb200

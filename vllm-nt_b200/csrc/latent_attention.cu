@@ -488,7 +488,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (active) buf[part * kMaxRows + r] = v;
       __syncwarp();
       if (lane == 0) mbar_arrive(exch);
-      const bool got = mbar_wait(exch, uses & 1, p.err);
+      const bool got = mbar_wait_warp(exch, uses & 1, p.err);
       ++uses;
       return got ? buf : nullptr;
     };
@@ -515,7 +515,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       for (int t = pc.t0; t < pc.t1; ++t, ++g) {
         const int s = g & 1;
         const int valid = pc.valid(t);
-        if (!mbar_wait(&bars[L::kSFull + s], (g / 2) & 1, p.err)) {
+        if (!mbar_wait_warp(&bars[L::kSFull + s], (g / 2) & 1, p.err)) {
           ok = false;
           break;
         }
@@ -573,7 +573,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           l_run += l2[0] + l2[1];
         }
         // P and O^T are free once the product of the tile before is complete
-        if (g >= 1 && !mbar_wait(&bars[L::kPvDone], (g - 1) & 1, p.err)) {
+        if (g >= 1 && !mbar_wait_warp(&bars[L::kPvDone], (g - 1) & 1, p.err)) {
           ok = false;
           break;
         }
@@ -622,7 +622,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       if (!ok) break;
       // O^T is final once the piece's last product is complete
-      ok = mbar_wait(&bars[L::kPvDone], (g - 1) & 1, p.err);
+      ok = mbar_wait_warp(&bars[L::kPvDone], (g - 1) & 1, p.err);
       const float* const all = ok ? exchange(l_run) : nullptr;
       if (all == nullptr) {
         ok = false;

@@ -1,0 +1,625 @@
+// Latent attention with the keys and values of every head expanded from the latent (prompts):
+//   s[i, j] = scale * (q_nope[i] . k_nope[j, h] + q_rope[i] . k_rope[j]),
+//   out[i, h] = sum_j softmax(s[i])_j v[j, h],   lse[i, h] = ln sum_j exp(s[i, j])
+// over each sequence's keys, causal masking aligned to their end.  q [tokens, heads, 192] is
+// [nope (128) | rope (64)]; the rotary key is one row a token for all heads and is read as it
+// is, never copied to the heads.
+//
+// Persistent, one CTA per SM, 384 threads.  A work item is 256 query rows of one head, as two
+// 128-row tiles A and B that share every K and V tile (128 keys) brought in:
+//   warps 0-3, 4-7  softmax of tile A, B: one thread a row.  The scores are read from TMEM
+//                   twice (maximum, then weights), so a thread never holds the row; the running
+//                   maximum is refreshed only when it grows by over 2^8 (the output is rescaled
+//                   then); weights go back to TMEM over the scores, rounded to the type.
+//   warp 8          S = Q K^T of A and B in turn (tcgen05, M = N = 128, twelve steps of 16).
+//   warp 9          O += P V (P from TMEM, V as it lies, MN-major, in two halves of 64 columns).
+//   warp 10         TMA: Q tiles and a ring of eight 16 KB chunks (128 rows x 64 columns) that
+//                   holds K_j (3), V_j (2), K_j+1 (3).
+// While one tile's softmax runs the tensor core works for the other.  TMEM: S_A, S_B, O_A, O_B,
+// 128 columns each.  Items are dealt round robin, a sequence's last (longest) rows first.
+// Bound: tensor core, 2 * 320 operations a visible (query, key) pair.
+#include <algorithm>
+
+#include "common.cuh"
+#include "tcgen05.cuh"
+
+namespace ntb200 {
+namespace {
+
+constexpr int kNope = 128, kRope = 64, kV = 128;
+constexpr int kQChunks = (kNope + kRope) / 64;  // 64-column chunks of a query or key row
+constexpr int kVChunks = kV / 64;
+constexpr int kBQ = 128, kBK = 128;
+constexpr int kItemRows = 2 * kBQ;
+constexpr int kChunkBytes = 128 * 128;  // 128 rows x 64 columns
+constexpr int kRing = 8;
+constexpr int kThreads = 384;
+constexpr int kSWarp = 8, kPvWarp = 9, kTmaWarp = 10, kAllocWarp = 11;
+constexpr float kRescaleLog2 = 8.0f;
+constexpr uint32_t kTmemCols = 512;
+constexpr uint32_t kTmemO = 256;  // S_A, S_B at 0, 128; O_A, O_B at 256, 384
+
+struct Smem {
+  static constexpr int kQ = 0;  // [2 tiles][3 chunks]
+  static constexpr int kKv = kQ + 2 * kQChunks * kChunkBytes;
+  static constexpr int kBars = kKv + kRing * kChunkBytes;
+  // indexes of the mbarriers
+  static constexpr int kQFull = 0, kQEmpty = 2, kFull = 4, kEmpty = kFull + kRing, kSFull = kEmpty + kRing,
+                       kPFull = kSFull + 2, kPvDone = kPFull + 2, kOFree = kPvDone + 2, kMmaDone = kOFree + 2,
+                       kNumBars = kMmaDone + 1;
+  static constexpr int kTmemBase = kBars + 8 * kNumBars;
+  static constexpr int kBytes = kTmemBase + 16;
+};
+static_assert(Smem::kBytes <= 227 * 1024, "shared memory");
+
+struct PrefillParams {
+  void* out;
+  float* lse;
+  const int32_t *cu_q, *cu_k;
+  int64_t o_tok, o_head, lse_tok;
+  int num_seqs, num_q, num_k, num_heads;
+  int causal;
+  float scale_log2;
+  unsigned int* err;
+};
+
+// 256 rows of one head: tile x has rows q0 + 128 x .. of the sequence (rows[x] of them) and
+// visits tiles[x] key tiles.
+struct Item {
+  int head, q_begin, q_len, k_begin, ctx, q0;
+  int rows[2], tiles[2];
+};
+
+// Walks a CTA's items (every role walks the same).  A warp holds 32 sequences' item counts at a
+// time and steps through the list as the item number grows.
+struct Walk {
+  int base;        // first sequence of the 32 held
+  int64_t before;  // items of the sequences before them
+  int64_t upto;    // this lane's inclusive count within the 32
+  int q_begin, q_len, k_begin, ctx;
+
+  __device__ __forceinline__ void load(const PrefillParams& p, int first) {
+    const int lane = threadIdx.x & 31;
+    const int b = first + lane;
+    base = first;
+    q_begin = q_len = k_begin = ctx = 0;
+    if (b < p.num_seqs) {
+      q_begin = p.cu_q[b];
+      k_begin = p.cu_k[b];
+      q_len = p.cu_q[b + 1] - q_begin;
+      ctx = p.cu_k[b + 1] - k_begin;
+      if (q_begin < 0 || q_len < 0 || q_len > p.num_q - q_begin || k_begin < 0 || ctx < 0 || ctx > p.num_k - k_begin) {
+        raise_device_error(p.err, NTB200_DEVERR_INDEX_RANGE);
+        q_begin = q_len = k_begin = ctx = 0;
+      }
+    }
+    upto = int64_t((q_len + kItemRows - 1) / kItemRows) * p.num_heads;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int64_t y = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o) upto += y;
+    }
+  }
+
+  __device__ __forceinline__ void begin(const PrefillParams& p) {
+    before = 0;
+    load(p, 0);
+  }
+
+  // item w (growing from call to call); false past the last one
+  __device__ __forceinline__ bool get(const PrefillParams& p, int64_t w, Item& it) {
+    for (;;) {
+      const int64_t all = __shfl_sync(0xffffffffu, upto, 31);
+      if (w < before + all) break;
+      if (base + 32 >= p.num_seqs) return false;
+      before += all;
+      load(p, base + 32);
+    }
+    const unsigned past = __ballot_sync(0xffffffffu, w < before + upto);
+    const int at = __ffs(past) - 1;
+    const int64_t prior = at > 0 ? __shfl_sync(0xffffffffu, upto, at - 1) : 0;
+    it.q_begin = __shfl_sync(0xffffffffu, q_begin, at);
+    it.q_len = __shfl_sync(0xffffffffu, q_len, at);
+    it.k_begin = __shfl_sync(0xffffffffu, k_begin, at);
+    it.ctx = __shfl_sync(0xffffffffu, ctx, at);
+    const int64_t i = w - before - prior;
+    const int block = int(i / p.num_heads);
+    it.head = int(i - int64_t(block) * p.num_heads);
+    const int blocks = (it.q_len + kItemRows - 1) / kItemRows;
+    it.q0 = (blocks - 1 - block) * kItemRows;
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+      const int first = it.q0 + x * kBQ;
+      it.rows[x] = min(max(it.q_len - first, 0), kBQ);
+      const int last = it.ctx - it.q_len + first + it.rows[x];
+      const int keys = it.rows[x] == 0 ? 0 : p.causal ? min(max(last, 0), it.ctx) : it.ctx;
+      it.tiles[x] = (keys + kBK - 1) / kBK;
+    }
+    return true;
+  }
+};
+
+__device__ __forceinline__ void umma_f16_tmem_a(uint32_t tmem_d, uint32_t tmem_a, uint64_t bdesc, uint32_t idesc,
+                                                uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(tmem_d),
+      "r"(tmem_a), "l"(bdesc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
+__device__ __forceinline__ void tmem_st_16(uint32_t taddr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+      "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
+      "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+
+__device__ __forceinline__ float hw_exp2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// The running maximum is subtracted less kBias: fp16 weights then span 2^7 .. 2^15 at the
+// row's largest score and reach 2^-31 of it before they vanish (bf16 has fp32's range).
+template <typename T>
+constexpr float kBias = 0.f;
+template <>
+constexpr float kBias<__half> = 7.f;
+
+template <typename T>
+__global__ void __launch_bounds__(kThreads, 1)
+    latent_prefill_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ CUtensorMap kn_map,
+                          const __grid_constant__ CUtensorMap kr_map, const __grid_constant__ CUtensorMap v_map,
+                          const PrefillParams p) {
+  extern __shared__ __align__(1024) uint8_t smem[];
+  const uint32_t sm = smem_u32(smem);
+  uint64_t* const bars = reinterpret_cast<uint64_t*>(smem + Smem::kBars);
+  uint32_t* const tmem_slot = reinterpret_cast<uint32_t*>(smem + Smem::kTmemBase);
+  const int warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31;
+  pdl_trigger();
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&bars[Smem::kQFull + i], 1);
+      mbar_init(&bars[Smem::kQEmpty + i], 1);
+      mbar_init(&bars[Smem::kSFull + i], 1);
+      mbar_init(&bars[Smem::kPFull + i], 4);  // one arrive a softmax warp
+      mbar_init(&bars[Smem::kPvDone + i], 1);
+      mbar_init(&bars[Smem::kOFree + i], 4);
+    }
+    for (int i = 0; i < kRing; ++i) mbar_init(&bars[Smem::kFull + i], 1), mbar_init(&bars[Smem::kEmpty + i], 1);
+    mbar_init(&bars[Smem::kMmaDone], 2);
+    fence_mbar_init();
+  }
+  pdl_wait();  // queries, keys and metadata come from the kernels before
+  if (warp == kAllocWarp) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
+                 "r"(kTmemCols)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  Walk walk;
+  Item it;
+  walk.begin(p);
+
+  if (warp == kTmaWarp) {
+    // ------------------------------ TMA producer ------------------------------
+    uint32_t nq[2] = {0, 0};  // Q tiles loaded
+    uint32_t n = 0;           // ring chunks loaded
+    bool ok = true;
+    for (int64_t w = blockIdx.x; ok && walk.get(p, w, it); w += gridDim.x) {
+      if (lane == 0) {
+        auto load_q = [&](int x) {
+          if (it.tiles[x] == 0) return;
+          uint64_t* const full = &bars[Smem::kQFull + x];
+          if (nq[x] >= 1 && !mbar_wait(&bars[Smem::kQEmpty + x], (nq[x] - 1) & 1, p.err)) {
+            ok = false;
+            return;
+          }
+          mbar_arrive_expect_tx(full, kQChunks * kChunkBytes);
+          for (int c = 0; c < kQChunks; ++c)
+            tma_load_3d(sm + Smem::kQ + (x * kQChunks + c) * kChunkBytes, &q_map, c * 64, it.head,
+                        it.q_begin + it.q0 + x * kBQ, smem_u32(full));
+          ++nq[x];
+        };
+        auto slot = [&]() -> uint64_t* {
+          const uint32_t s = n % kRing;
+          if (n >= kRing && !mbar_wait(&bars[Smem::kEmpty + s], (n / kRing - 1) & 1, p.err)) {
+            ok = false;
+            return nullptr;
+          }
+          mbar_arrive_expect_tx(&bars[Smem::kFull + s], kChunkBytes);
+          return &bars[Smem::kFull + s];
+        };
+        const int tiles = max(it.tiles[0], it.tiles[1]);
+        load_q(0);
+        for (int j = 0; ok && j < tiles; ++j) {
+          const int row = it.k_begin + j * kBK;
+          for (int c = 0; ok && c < kQChunks; ++c) {
+            uint64_t* const full = slot();
+            if (full == nullptr) break;
+            const uint32_t dst = sm + Smem::kKv + (n % kRing) * kChunkBytes;
+            if (c < kNope / 64) tma_load_3d(dst, &kn_map, c * 64, it.head, row, smem_u32(full));
+            else tma_load_2d(dst, &kr_map, 0, row, smem_u32(full));
+            ++n;
+          }
+          if (ok && j == 0) load_q(1);
+          for (int c = 0; ok && c < kVChunks; ++c) {
+            uint64_t* const full = slot();
+            if (full == nullptr) break;
+            tma_load_3d(sm + Smem::kKv + (n % kRing) * kChunkBytes, &v_map, c * 64, it.head, row, smem_u32(full));
+            ++n;
+          }
+        }
+      }
+      ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
+    }
+    if (lane == 0) {
+      // drain the copies that may still be in flight
+      for (int x = 0; x < 2; ++x)
+        if (nq[x] > 0) mbar_wait(&bars[Smem::kQFull + x], (nq[x] - 1) & 1, p.err);
+      for (uint32_t i = n > kRing ? n - kRing : 0; i < n; ++i)
+        mbar_wait(&bars[Smem::kFull + i % kRing], (i / kRing) & 1, p.err);
+    }
+  } else if (warp == kSWarp) {
+    // -------------------------- MMA issuer: S = Q K^T --------------------------
+    const uint32_t idesc = make_idesc(std::is_same<T, __nv_bfloat16>::value, kBQ, kBK);
+    uint32_t ns[2] = {0, 0};  // products issued a tile
+    uint32_t nq[2] = {0, 0};
+    uint32_t n = 0;  // ring chunks passed (V's among them)
+    bool ok = true;
+    for (int64_t w = blockIdx.x; ok && walk.get(p, w, it); w += gridDim.x) {
+      if (lane == 0) {
+        const int tiles = max(it.tiles[0], it.tiles[1]);
+        for (int j = 0; ok && j < tiles; ++j, n += kQChunks + kVChunks) {
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            if (!ok || j >= it.tiles[x]) continue;
+            const bool last_user = x == 1 || j >= it.tiles[1];
+            // the buffer's weights of the tile before have been used up
+            if ((j == 0 && !mbar_wait(&bars[Smem::kQFull + x], nq[x] & 1, p.err)) ||
+                (ns[x] >= 1 && !mbar_wait(&bars[Smem::kPvDone + x], (ns[x] - 1) & 1, p.err))) {
+              ok = false;
+              continue;
+            }
+            for (int c = 0; c < kQChunks; ++c) {
+              const uint32_t s = (n + c) % kRing;
+              if (!mbar_wait(&bars[Smem::kFull + s], ((n + c) / kRing) & 1, p.err)) {
+                ok = false;
+                break;
+              }
+              tc_fence_after();
+              const uint64_t a = sw128_kmajor_desc(sm + Smem::kQ + (x * kQChunks + c) * kChunkBytes);
+              const uint64_t b = sw128_kmajor_desc(sm + Smem::kKv + s * kChunkBytes);
+#pragma unroll
+              for (int k = 0; k < 4; ++k) umma_f16(tmem + x * kBK, a + 2 * k, b + 2 * k, idesc, (c | k) ? 1u : 0u);
+              if (last_user) umma_commit(&bars[Smem::kEmpty + s]);
+            }
+            umma_commit(&bars[Smem::kSFull + x]);
+            ++ns[x];
+            if (j + 1 == it.tiles[x]) {
+              umma_commit(&bars[Smem::kQEmpty + x]);
+              ++nq[x];
+            }
+          }
+        }
+      }
+      ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
+    }
+    if (lane == 0) {
+      // every issued MMA completes before TMEM may be released
+      umma_commit(&bars[Smem::kMmaDone]);
+      mbar_wait(&bars[Smem::kMmaDone], 0, p.err);
+    }
+  } else if (warp == kPvWarp) {
+    // -------------------------- MMA issuer: O += P V --------------------------
+    const uint32_t idesc = make_idesc(std::is_same<T, __nv_bfloat16>::value, kBQ, 64) | (1u << 16);  // B (V) MN-major
+    uint32_t np[2] = {0, 0};     // products issued a tile
+    uint32_t items[2] = {0, 0};  // outputs begun
+    uint32_t n = 0;
+    bool ok = true;
+    for (int64_t w = blockIdx.x; ok && walk.get(p, w, it); w += gridDim.x) {
+      if (lane == 0) {
+        const int tiles = max(it.tiles[0], it.tiles[1]);
+        for (int j = 0; ok && j < tiles; ++j, n += kQChunks + kVChunks) {
+          const int steps = (min(it.ctx - j * kBK, kBK) + 15) / 16;
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            if (!ok || j >= it.tiles[x]) continue;
+            const bool last_user = x == 1 || j >= it.tiles[1];
+            if (!mbar_wait(&bars[Smem::kPFull + x], np[x] & 1, p.err) ||
+                (j == 0 && items[x] >= 1 && !mbar_wait(&bars[Smem::kOFree + x], (items[x] - 1) & 1, p.err))) {
+              ok = false;
+              continue;
+            }
+            for (int c = 0; c < kVChunks; ++c) {
+              const uint32_t at = n + kQChunks + c, s = at % kRing;
+              if (!mbar_wait(&bars[Smem::kFull + s], (at / kRing) & 1, p.err)) {
+                ok = false;
+                break;
+              }
+              tc_fence_after();
+              const uint32_t vb = sm + Smem::kKv + s * kChunkBytes;
+              for (int k = 0; k < steps; ++k)
+                umma_f16_tmem_a(tmem + kTmemO + x * kV + c * 64, tmem + x * kBK + k * 8,
+                                sw128_mnmajor_desc(vb + k * 2048, kChunkBytes), idesc, (j > 0 || k > 0) ? 1u : 0u);
+              if (last_user) umma_commit(&bars[Smem::kEmpty + s]);
+            }
+            umma_commit(&bars[Smem::kPvDone + x]);
+            ++np[x];
+            if (j == 0) ++items[x];
+          }
+        }
+      }
+      ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
+    }
+    if (lane == 0) {
+      umma_commit(&bars[Smem::kMmaDone]);
+      mbar_wait(&bars[Smem::kMmaDone], 0, p.err);
+    }
+  } else if (warp < 8) {
+    // ------------------------------ softmax + output ------------------------------
+    const int x = warp >> 2;
+    const int r = (warp & 3) * 32 + lane;
+    const uint32_t lanes = uint32_t((warp & 3) * 32) << 16;
+    const uint32_t s_tmem = tmem + x * kBK + lanes;
+    const uint32_t o_tmem = tmem + kTmemO + x * kV + lanes;
+    uint32_t g = 0;  // key tiles done
+    uint32_t n = 0;  // ring chunks passed
+    bool ok = true;
+    for (int64_t w = blockIdx.x; ok && walk.get(p, w, it); w += gridDim.x) {
+      const int qi = it.q0 + x * kBQ + r;
+      const bool there = r < it.rows[x];
+      const int64_t tok = it.q_begin + qi;
+      T* const orow = static_cast<T*>(p.out) + tok * p.o_tok + int64_t(it.head) * p.o_head;
+      const int tiles = it.tiles[x];
+      const int both = max(it.tiles[0], it.tiles[1]);
+      if (tiles == 0) {  // no visible key: zero rows, as for an empty softmax
+        if (there) {
+#pragma unroll
+          for (int c = 0; c < kV / 8; ++c) reinterpret_cast<uint4*>(orow)[c] = make_uint4(0u, 0u, 0u, 0u);
+          if (p.lse != nullptr) p.lse[tok * p.lse_tok + it.head] = -INFINITY;
+        }
+        n += both * (kQChunks + kVChunks);
+        continue;
+      }
+      // this row sees keys [0, limit)
+      const int limit = !there ? 0 : p.causal ? min(max(it.ctx - it.q_len + qi + 1, 0), it.ctx) : it.ctx;
+      float m = -INFINITY, l = 0.f;
+      for (int j = 0; j < tiles; ++j, ++g) {
+        if (!mbar_wait_warp(&bars[Smem::kSFull + x], g & 1, p.err)) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        const int seen = limit - j * kBK;  // columns i < seen are visible
+        // ---- the tile's maximum ----
+        float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+        for (int c = 0; c < kBK / 32; ++c) {
+          uint32_t v[32];
+          __syncwarp();
+          tmem_ld_32(s_tmem + c * 32, v);
+          if (seen >= (c + 1) * 32) {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) m4[i & 3] = fmaxf(m4[i & 3], __uint_as_float(v[i]));
+          } else {
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+              m4[i & 3] = fmaxf(m4[i & 3], c * 32 + i < seen ? __uint_as_float(v[i]) : -INFINITY);
+          }
+        }
+        // (the scale is positive, so the largest score is the largest scaled one)
+        const float top = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * p.scale_log2;
+        const float m_new = fmaxf(m, top);
+        const bool up = m_new > m + kRescaleLog2;  // also true for the first finite maximum
+        if (__any_sync(0xffffffffu, up)) {
+          const float alpha = up ? hw_exp2(m - m_new) : 1.f;
+          if (up) m = m_new;
+          l *= alpha;
+          if (j > 0) {
+            if (!mbar_wait_warp(&bars[Smem::kPvDone + x], (g - 1) & 1, p.err)) {
+              ok = false;
+              break;
+            }
+            tc_fence_after();
+#pragma unroll
+            for (int c = 0; c < kV / 16; ++c) {
+              uint32_t v[16];
+              __syncwarp();
+              tmem_ld_16(o_tmem + c * 16, v);
+#pragma unroll
+              for (int i = 0; i < 16; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) * alpha);
+              tmem_st_16(o_tmem + c * 16, v);
+            }
+          }
+        }
+        // ---- the weights, over the scores they come from ----
+        const float m_use = m == -INFINITY ? 0.f : m - kBias<T>;
+        float l4[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int c = 0; c < kBK / 32; ++c) {
+          uint32_t v[32], pk[16];
+          __syncwarp();
+          tmem_ld_32(s_tmem + c * 32, v);
+          float e[32];
+          if (seen >= (c + 1) * 32) {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) e[i] = hw_exp2(fmaf(__uint_as_float(v[i]), p.scale_log2, -m_use));
+          } else {
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+              e[i] = c * 32 + i < seen ? hw_exp2(fmaf(__uint_as_float(v[i]), p.scale_log2, -m_use)) : 0.f;
+          }
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            l4[i & 3] += e[2 * i] + e[2 * i + 1];
+            Pair<T>::store(reinterpret_cast<T*>(&pk[i]), e[2 * i], e[2 * i + 1]);
+          }
+          tmem_st_16(s_tmem + c * 16, pk);
+        }
+        l += (l4[0] + l4[1]) + (l4[2] + l4[3]);
+        asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+        const int inside = it.ctx - j * kBK;  // rows of this V tile that belong to the sequence
+        if (inside < kBK && (inside & 15) != 0) {
+          // rows behind the sequence, up to the product's next step of 16, are another's: zeroed,
+          // so that a weight of 0 never meets a non-finite value
+          const int stop = (inside + 15) & ~15;
+#pragma unroll
+          for (int c = 0; c < kVChunks; ++c) {
+            const uint32_t at = n + kQChunks + c, s = at % kRing;
+            if (!mbar_wait_warp(&bars[Smem::kFull + s], (at / kRing) & 1, p.err)) ok = false;
+            for (int i = r; i < (stop - inside) * 8; i += kBQ)
+              *reinterpret_cast<uint4*>(smem + Smem::kKv + s * kChunkBytes + (inside + (i >> 3)) * 128 + (i & 7) * 16) =
+                  make_uint4(0u, 0u, 0u, 0u);
+          }
+          fence_proxy_async_smem();
+          if (!ok) break;
+        }
+        n += kQChunks + kVChunks;
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bars[Smem::kPFull + x]);
+      }
+      if (!ok) break;
+      n += (both - tiles) * (kQChunks + kVChunks);
+      // the item's last product is complete: O is final
+      ok = mbar_wait_warp(&bars[Smem::kPvDone + x], (g - 1) & 1, p.err);
+      if (!ok) break;
+      tc_fence_after();
+      const float inv = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll
+      for (int c = 0; c < kV / 32; ++c) {
+        uint32_t v[32];
+        __syncwarp();
+        tmem_ld_32(o_tmem + c * 32, v);
+        if (there) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            float f[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) f[e] = l == 0.f ? 0.f : __uint_as_float(v[i * 8 + e]) * inv;
+            *reinterpret_cast<Vec<T, 8>*>(orow + c * 32 + i * 8) = pack_f<T, 8>(f);
+          }
+        }
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&bars[Smem::kOFree + x]);  // the next item may overwrite O
+      if (there && p.lse != nullptr)
+        p.lse[tok * p.lse_tok + it.head] = l == 0.f ? -INFINITY : (m - kBias<T> + log2f(l)) * 0.6931471805599453f;
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (warp == kAllocWarp) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols) : "memory");
+  }
+}
+
+// rows [tokens, heads, dim] (or [tokens, dim], heads 0): box = 128 tokens x one head x 64 columns
+int make_rows_map(CUtensorMap* map, const void* base, bool bf16, int64_t dim, int64_t tokens, int64_t heads,
+                  int64_t tok_stride, int64_t head_stride) {
+  EncodeTiledFn enc = encode_fn();
+  if (enc == nullptr) return fail(NTB200_ERR_CUDA, "cuTensorMapEncodeTiled unavailable");
+  const cuuint64_t tok = cuuint64_t((tokens > 1 ? tok_stride : dim) * 2);
+  const cuuint64_t dims3[3] = {cuuint64_t(dim), cuuint64_t(heads), cuuint64_t(tokens)};
+  const cuuint64_t strides3[2] = {cuuint64_t((heads > 1 ? head_stride : dim) * 2), tok};
+  const cuuint32_t box3[3] = {64, 1, 128};
+  const cuuint64_t dims2[2] = {cuuint64_t(dim), cuuint64_t(tokens)};
+  const cuuint64_t strides2[1] = {tok};
+  const cuuint32_t box2[2] = {64, 128};
+  const cuuint32_t estr[3] = {1, 1, 1};
+  const CUresult r = enc(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
+                         heads > 0 ? 3 : 2, const_cast<void*>(base), heads > 0 ? dims3 : dims2,
+                         heads > 0 ? strides3 : strides2, heads > 0 ? box3 : box2, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                         CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fail(NTB200_ERR_CUDA, "cuTensorMapEncodeTiled (latent prefill) failed (%d)", int(r));
+  return NTB200_OK;
+}
+
+template <typename T>
+int launch_prefill(const CUtensorMap& q, const CUtensorMap& kn, const CUtensorMap& kr, const CUtensorMap& v,
+                   const PrefillParams& p, int64_t ctas, int slot, cudaStream_t s) {
+  const int st = ensure_smem_attribute(reinterpret_cast<const void*>(latent_prefill_kernel<T>), Smem::kBytes, slot);
+  if (st != NTB200_OK) return st;
+  return launch_kernel("latent_attention_prefill", latent_prefill_kernel<T>, dim3(unsigned(ctas)), dim3(kThreads),
+                       Smem::kBytes, s, q, kn, kr, v, p);
+}
+
+}  // namespace
+}  // namespace ntb200
+
+extern "C" int ntb200_latent_attention_prefill(
+    void* out, float* lse, const void* query, const void* k_nope, const void* k_rope, const void* value,
+    const int32_t* cu_seqlens_q, const int32_t* cu_seqlens_k, int64_t num_seqs, int64_t num_q_tokens,
+    int64_t num_k_tokens, int64_t num_heads, int64_t nope_dim, int64_t rope_dim, int64_t v_dim, int64_t max_query_len,
+    float scale, int causal, int64_t q_token_stride, int64_t q_head_stride, int64_t kn_token_stride,
+    int64_t kn_head_stride, int64_t kr_token_stride, int64_t v_token_stride, int64_t v_head_stride,
+    int64_t out_token_stride, int64_t out_head_stride, int64_t lse_token_stride, int dtype, void* stream) {
+  using namespace ntb200;
+  if (dtype != NTB200_DTYPE_BF16 && dtype != NTB200_DTYPE_F16)
+    return fail(NTB200_ERR_UNSUPPORTED_DTYPE, "latent_attention_prefill: dtype %d (bf16/f16 only)", dtype);
+  if (nope_dim != kNope || rope_dim != kRope || v_dim != kV)
+    return fail(NTB200_ERR_UNSUPPORTED_SHAPE,
+                "latent_attention_prefill: nope_dim %lld / rope_dim %lld / v_dim %lld (128 / 64 / 128 only)",
+                (long long)nope_dim, (long long)rope_dim, (long long)v_dim);
+  if (num_seqs < 0 || num_q_tokens < 0 || num_k_tokens < 0 || num_heads <= 0 || max_query_len < 0)
+    return fail(NTB200_ERR_INVALID_ARGUMENT, "latent_attention_prefill: bad sizes");
+  if (!(scale > 0.f))
+    return fail(NTB200_ERR_INVALID_ARGUMENT, "latent_attention_prefill: scale must be positive");
+  if (num_seqs == 0 || num_q_tokens == 0 || max_query_len == 0) return NTB200_OK;
+  if (num_seqs > 0x7fffffff - 32 || num_q_tokens > 0x7fffffff || num_k_tokens > 0x7fffffff || num_heads > 65535)
+    return fail(NTB200_ERR_UNSUPPORTED_SHAPE, "latent_attention_prefill: sizes beyond the launch limits");
+  if (!out || !query || !cu_seqlens_q || !cu_seqlens_k || (num_k_tokens > 0 && (!k_nope || !k_rope || !value)))
+    return fail(NTB200_ERR_INVALID_ARGUMENT, "latent_attention_prefill: null pointer");
+  if (!aligned16(out) || !aligned16(query) || !aligned16(k_nope) || !aligned16(k_rope) || !aligned16(value) ||
+      q_token_stride % 8 || q_head_stride % 8 || kn_token_stride % 8 || kn_head_stride % 8 || kr_token_stride % 8 ||
+      v_token_stride % 8 || v_head_stride % 8 || out_token_stride % 8 || out_head_stride % 8)
+    return fail(NTB200_ERR_MISALIGNED, "latent_attention_prefill: pointers 16-byte aligned, strides multiples of 8");
+  const bool bf16 = dtype == NTB200_DTYPE_BF16;
+  CUtensorMap q, kn, kr, v;
+  int st = make_rows_map(&q, query, bf16, kNope + kRope, num_q_tokens, num_heads, q_token_stride, q_head_stride);
+  if (st != NTB200_OK) return st;
+  kn = kr = v = q;  // never read when there are no keys
+  if (num_k_tokens > 0) {
+    st = make_rows_map(&kn, k_nope, bf16, kNope, num_k_tokens, num_heads, kn_token_stride, kn_head_stride);
+    if (st == NTB200_OK) st = make_rows_map(&kr, k_rope, bf16, kRope, num_k_tokens, 0, kr_token_stride, 0);
+    if (st == NTB200_OK) st = make_rows_map(&v, value, bf16, kV, num_k_tokens, num_heads, v_token_stride, v_head_stride);
+    if (st != NTB200_OK) return st;
+  }
+  PrefillParams p = {};
+  p.out = out;
+  p.lse = lse;
+  p.cu_q = cu_seqlens_q;
+  p.cu_k = cu_seqlens_k;
+  p.o_tok = out_token_stride;
+  p.o_head = out_head_stride;
+  p.lse_tok = lse_token_stride;
+  p.num_seqs = int(num_seqs);
+  p.num_q = int(num_q_tokens);
+  p.num_k = int(num_k_tokens);
+  p.num_heads = int(num_heads);
+  p.causal = causal != 0;
+  p.scale_log2 = scale * 1.4426950408889634f;  // softmax in the exp2 domain
+  p.err = device_error_word();
+  // no more CTAs than there can be items: every sequence rounds up at most once
+  const int64_t by_len = ceil_div(std::min(max_query_len, num_q_tokens), kItemRows) * num_seqs;
+  const int64_t by_tokens = ceil_div(num_q_tokens, kItemRows) + num_seqs;
+  const int64_t ctas = std::min<int64_t>(std::min(by_len, by_tokens) * num_heads, num_sms());
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  return bf16 ? launch_prefill<__nv_bfloat16>(q, kn, kr, v, p, ctas, 134, s)
+              : launch_prefill<__half>(q, kn, kr, v, p, ctas, 135, s);
+}

@@ -921,6 +921,60 @@ void latent_attention(at::Tensor out, const std::optional<at::Tensor>& lse, cons
         op);
 }
 
+// Latent attention over expanded per-head keys and values, the rotary key shared by the heads.
+void latent_attention_prefill(at::Tensor out, const std::optional<at::Tensor>& lse, const at::Tensor& query,
+                              const at::Tensor& k_nope, const at::Tensor& k_rope, const at::Tensor& value,
+                              const at::Tensor& cu_seqlens_q, const at::Tensor& cu_seqlens_k, int64_t max_query_len,
+                              double scale, bool causal) {
+  const char* op = "latent_attention_prefill";
+  require_cuda(query, "query");
+  same_device(query, out, op);
+  same_device(query, k_nope, op);
+  same_device(query, k_rope, op);
+  same_device(query, value, op);
+  same_device(query, cu_seqlens_q, op);
+  same_device(query, cu_seqlens_k, op);
+  const auto dt = query.scalar_type();
+  TORCH_CHECK(query.dim() == 3 && query.stride(2) == 1 && k_nope.dim() == 3 && k_nope.stride(2) == 1 &&
+                  value.dim() == 3 && value.stride(2) == 1 && k_rope.dim() == 2 && k_rope.stride(1) == 1,
+              "ntb200.latent_attention_prefill: query, k_nope, value [tokens, heads, dim], k_rope [tokens, dim]");
+  const int64_t tq = query.size(0), h = query.size(1), tk = k_nope.size(0);
+  TORCH_CHECK(k_nope.size(1) == h && value.size(1) == h && value.size(0) == tk && k_rope.size(0) == tk &&
+                  query.size(2) == k_nope.size(2) + k_rope.size(1),
+              "ntb200.latent_attention_prefill: query [q, heads, nope + rope], k_nope [k, heads, nope], k_rope [k, rope], "
+              "value [k, heads, v]");
+  TORCH_CHECK(out.dim() == 3 && out.size(0) == tq && out.size(1) == h && out.size(2) == value.size(2) &&
+                  out.stride(2) == 1,
+              "ntb200.latent_attention_prefill: out must be [q, heads, v]");
+  TORCH_CHECK(k_nope.scalar_type() == dt && k_rope.scalar_type() == dt && value.scalar_type() == dt &&
+                  out.scalar_type() == dt,
+              "ntb200.latent_attention_prefill: tensors of one dtype");
+  TORCH_CHECK(cu_seqlens_q.scalar_type() == at::kInt && cu_seqlens_k.scalar_type() == at::kInt &&
+                  cu_seqlens_q.is_contiguous() && cu_seqlens_k.is_contiguous() && cu_seqlens_q.dim() == 1 &&
+                  cu_seqlens_q.numel() >= 1 && cu_seqlens_k.dim() == 1 && cu_seqlens_k.numel() == cu_seqlens_q.numel(),
+              "ntb200.latent_attention_prefill: cu_seqlens_q/k must be int32 contiguous [seqs + 1]");
+  float* l = nullptr;
+  int64_t ls = 0;
+  if (lse.has_value()) {
+    same_device(query, *lse, op);
+    TORCH_CHECK(lse->scalar_type() == at::kFloat && lse->dim() == 2 && lse->size(0) == tq && lse->size(1) == h &&
+                    (h == 1 || lse->stride(1) == 1),
+                "ntb200.latent_attention_prefill: lse must be float32 [q, heads]");
+    l = lse->data_ptr<float>();
+    ls = lse->stride(0);
+  }
+  const auto ts = [](const at::Tensor& t) { return t.size(0) > 1 ? t.stride(0) : 0; };
+  const auto hs = [](const at::Tensor& t) { return t.size(1) > 1 ? t.stride(1) : 0; };
+  c10::cuda::CUDAGuard guard(query.device());
+  check(ntb200_latent_attention_prefill(
+            out.data_ptr(), l, query.data_ptr(), k_nope.data_ptr(), k_rope.data_ptr(), value.data_ptr(),
+            cu_seqlens_q.data_ptr<int32_t>(), cu_seqlens_k.data_ptr<int32_t>(), cu_seqlens_q.numel() - 1, tq, tk, h,
+            k_nope.size(2), k_rope.size(1), value.size(2), max_query_len, static_cast<float>(scale), causal ? 1 : 0,
+            ts(query), hs(query), ts(k_nope), hs(k_nope), ts(k_rope), ts(value), hs(value), ts(out), hs(out), ls,
+            dtype_code(query), stream_of(query)),
+        op);
+}
+
 }  // namespace
 
 TORCH_LIBRARY(ntb200, m) {
@@ -1006,6 +1060,9 @@ TORCH_LIBRARY(ntb200, m) {
       "latent_attention(Tensor(a!) out, Tensor(b!)? lse, Tensor q_latent, Tensor q_rope, Tensor kv_cache, "
       "Tensor? query_start_loc, Tensor seq_lens, Tensor block_table, int max_query_len, int max_seq_len, "
       "float scale, Tensor(c!)? workspace) -> ()");
+  m.def(
+      "latent_attention_prefill(Tensor(a!) out, Tensor(b!)? lse, Tensor query, Tensor k_nope, Tensor k_rope, "
+      "Tensor value, Tensor cu_seqlens_q, Tensor cu_seqlens_k, int max_query_len, float scale, bool causal) -> ()");
 }
 
 TORCH_LIBRARY_IMPL(ntb200, CUDA, m) {
@@ -1038,4 +1095,5 @@ TORCH_LIBRARY_IMPL(ntb200, CUDA, m) {
   m.impl("rope_cos_sin_cache", &rope_cos_sin_cache);
   m.impl("latent_rope_and_cache", &latent_rope_and_cache);
   m.impl("latent_attention", &latent_attention);
+  m.impl("latent_attention_prefill", &latent_attention_prefill);
 }

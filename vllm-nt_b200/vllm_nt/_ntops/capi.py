@@ -115,6 +115,9 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
         c_int,
         [c_void_p] * 8 + [c_int64] * 11 + [c_float] + [c_int64] * 9 + [c_void_p, c_size_t, c_int, c_void_p],
     ),
+    "ntb200_latent_attention_prefill": (
+        c_int, [c_void_p] * 8 + [c_int64] * 8 + [c_float, c_int] + [c_int64] * 10 + [c_int, c_void_p]
+    ),
     "ntb200_linear_workspace_size": (c_size_t, [c_int64, c_int64, c_int64]),
     "ntb200_linear": (
         c_int,

@@ -7,7 +7,12 @@ from vllm_nt._ntops.torch.attention import (
 )
 from vllm_nt._ntops.torch.embedding import embedding
 from vllm_nt._ntops.torch.kv_cache import get_kv_from_cache, store_kvcache
-from vllm_nt._ntops.torch.latent import latent_attention, latent_rope_and_cache, latent_workspace_bytes
+from vllm_nt._ntops.torch.latent import (
+    latent_attention,
+    latent_attention_prefill,
+    latent_rope_and_cache,
+    latent_workspace_bytes,
+)
 from vllm_nt._ntops.torch.linear import linear, matmul
 from vllm_nt._ntops.torch.rms_norm import fused_add_rms_norm, rms_norm
 from vllm_nt._ntops.torch.sampler import apply_top_k_top_p, random_sample
@@ -28,6 +33,7 @@ __all__ = [
     "fused_add_rms_norm",
     "get_kv_from_cache",
     "latent_attention",
+    "latent_attention_prefill",
     "latent_rope_and_cache",
     "latent_workspace_bytes",
     "linear",

@@ -53,6 +53,7 @@ def _register_fakes() -> None:
         "rope_cos_sin_cache",
         "latent_rope_and_cache",
         "latent_attention",
+        "latent_attention_prefill",
     ):
         torch.library.register_fake(f"ntb200::{name}")(nothing)
 

@@ -77,3 +77,29 @@ def latent_attention(
     ops().latent_attention(out, lse, q_latent, q_rope, kv_cache, query_start_loc, seq_lens.contiguous(), block_table,
                            most, int(max_seq_len or 0), float(scale), workspace)
     return out
+
+
+def latent_attention_prefill(
+    out: torch.Tensor,
+    query: torch.Tensor,
+    k_nope: torch.Tensor,
+    k_rope: torch.Tensor,
+    value: torch.Tensor,
+    cu_seqlens_q: torch.Tensor,
+    cu_seqlens_k: torch.Tensor,
+    max_query_len: int,
+    scale: float,
+    causal: bool = True,
+    lse: torch.Tensor | None = None,
+) -> torch.Tensor:
+    """Varlen attention over keys and values expanded from the latent: query [Tq, heads, 192],
+    k_nope and value [Tk, heads, 128] (slices of the up-projection's rows go in as they are),
+    k_rope [Tk, 64] shared by the heads, out [Tq, heads, 128]; sequence b's queries and keys at
+    rows cu_seqlens_q[b] .. [b + 1] and cu_seqlens_k[b] .. [b + 1], causal masking aligned to the
+    end of its keys.  ``lse`` float32 [Tq, heads] receives the natural log of the softmax sums,
+    with which two parts of a context can be merged."""
+    cu_q = cu_seqlens_q if cu_seqlens_q.dtype == torch.int32 else cu_seqlens_q.to(torch.int32)
+    cu_k = cu_seqlens_k if cu_seqlens_k.dtype == torch.int32 else cu_seqlens_k.to(torch.int32)
+    ops().latent_attention_prefill(out, lse, query, k_nope, k_rope, value, cu_q.contiguous(), cu_k.contiguous(),
+                                   int(max_query_len), float(scale), bool(causal))
+    return out
