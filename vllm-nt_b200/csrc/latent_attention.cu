@@ -13,17 +13,22 @@
 // the shares.  When a sequence has several groups (up to kMaxTeams), CTA c takes group
 // c % groups only: neighbours read the same tiles at the same time, the second from L2.
 //
-// One tile, 640 threads:
-//   warp 0      TMA: the item's queries (9 chunks of 64 columns), then per tile the rotary
-//               chunk and 4 pairs of latent chunks into two rings, page by page.
-//   warp 1      S = Q C^T on tcgen05 (M = 128: rows past the group's are whatever shared memory
-//               holds, and their lanes are never read; N = 64 tokens), two S buffers.
-//   warp 2      O^T += C^T P^T: the cached rows as the MN-major A operand (M = 128 latent
-//               columns, four times), P [rows, tokens] as B.  O^T takes 4 x rows TMEM columns
-//               where O would need all 512, which leaves room for S and lets the tile that S
-//               was made from be used as it lies.
-//   warps 4-19  softmax (a lane a query row, 16 of the tile's tokens a warp), the running max
-//               refreshed only when it grows by over 2^8 (O^T is rescaled then), the output.
+// One tile, 256 threads:
+//   warp 0     TMA: the item's queries (9 chunks of 64 columns), then units of 16 cached tokens
+//              into a ring of 8.  A unit is one copy of a 5-D box (64 columns, 8 tokens, 9 chunks,
+//              2 groups of 8 tokens): whole rows are asked for together, and they land as the
+//              1024-byte swizzled atoms that the MMAs read, [8-token group][chunk].
+//   warp 1     S = Q C^T on tcgen05 (M = 64: rows past the group's are whatever shared memory
+//              holds, and their lanes are never used; N = 64 tokens), two S buffers.
+//   warp 2     O^T += C^T P^T: the cached rows as the MN-major A operand (M = 128 latent
+//              columns, four times), P [rows, tokens] as B.  O^T takes 4 x rows TMEM columns
+//              where O would need all 512, which leaves room for S and lets the tile that S
+//              was made from be used as it lies.  A unit is free after its 16-token step.
+//   warps 4-7  softmax: a warp the 16 rows of its TMEM lanes, four lanes a row, so a row's
+//              maximum is two shuffles; refreshed only when it grows by over 2^8 (O^T is
+//              rescaled then); and the output.
+// The issuing warps stay converged and elect the lane for each instruction: descriptors then live
+// in uniform registers (from a branch on one lane an MMA took 52 cycles to issue, so 48).
 //
 // Bound: HBM while 2 * rows * 1088 operations a token take less time than its 1152 bytes.
 #include <algorithm>
@@ -38,43 +43,40 @@ constexpr int kLatent = 512;
 constexpr int kRope = 64;
 constexpr int kChunks = (kLatent + kRope) / 64;  // 64-column chunks of a row; the last is rotary
 constexpr int kTile = 64;                        // cached tokens a tile
-constexpr int kChunkBytes = kTile * 128;         // 64 tokens x 64 columns
-constexpr int kPairBytes = 2 * kChunkBytes;
-constexpr int kPairs = kLatent / 128;
+constexpr int kUnit = 16;                        // cached tokens a copy, and an O^T step
+constexpr int kGroupBytes = kChunks * 1024;      // 8 tokens: one 1024-byte atom a chunk
+constexpr int kUnitBytes = 2 * kGroupBytes;
+constexpr int kTileUnits = kTile / kUnit;
+constexpr int kRing = 2 * kTileUnits;            // units
+constexpr int kMTiles = kLatent / 128;           // M = 128 products that make up O^T
 constexpr int kMaxRows = 64;                     // query rows a group
-constexpr int kSmWarps = 16;
 constexpr int kFirstSmWarp = 4;
-constexpr int kThreads = 32 * (kFirstSmWarp + kSmWarps);
-constexpr int kParts = 4;                        // warps that share a row's 64 tokens
-constexpr int kPartCols = kTile / kParts;
+constexpr int kSmThreads = 128;
+constexpr int kThreads = 32 * kFirstSmWarp + kSmThreads;
 constexpr int kMaxTeams = 8;
 constexpr float kRescaleLog2 = 8.0f;
 
 template <int N>
 struct Layout {
   static constexpr int kQBufs = N == 64 ? 1 : 2;
-  static constexpr int kRopeSlots = 2;
-  static constexpr int kPairSlots = N == 16 ? 10 : 8;
   static constexpr int kQBytes = kChunks * N * 128;
   static constexpr int kQ = 0;
-  static constexpr int kRopeRing = kQ + kQBufs * kQBytes;
-  static constexpr int kPairRing = kRopeRing + kRopeSlots * kChunkBytes;
-  static constexpr int kP = kPairRing + kPairSlots * kPairBytes;
-  static constexpr int kRed = kP + N * 128;                       // [2][kParts][64] floats
-  static constexpr int kBars = kRed + 2 * kParts * kMaxRows * 4;  // mbarriers
-  static constexpr int kQFull = 0, kQEmpty = kQFull + kQBufs, kRopeFull = kQEmpty + kQBufs,
-                       kRopeEmpty = kRopeFull + kRopeSlots, kPairFull = kRopeEmpty + kRopeSlots,
-                       kPairEmpty = kPairFull + kPairSlots, kSFull = kPairEmpty + kPairSlots, kSFree = kSFull + 2,
-                       kPFull = kSFree + 2, kPvDone = kPFull + 1, kOFree = kPvDone + 1, kMmaDone = kOFree + 1,
-                       kExch = kMmaDone + 1, kNumBars = kExch + 1;
+  static constexpr int kKv = kQ + kQBufs * kQBytes;
+  static constexpr int kP = kKv + kRing * kUnitBytes;
+  static constexpr int kRowF = kP + N * 128;           // [64] floats: a row's rescale, then 1 / sum
+  static constexpr int kRowAt = kRowF + kMaxRows * 4;  // [64] int64: where a row's output goes
+  static constexpr int kBars = kRowAt + kMaxRows * 8;  // mbarriers
+  static constexpr int kQFull = 0, kQEmpty = kQFull + kQBufs, kFull = kQEmpty + kQBufs, kEmpty = kFull + kRing,
+                       kSFull = kEmpty + kRing, kSFree = kSFull + 2, kPFull = kSFree + 2, kPvDone = kPFull + 1,
+                       kOFree = kPvDone + 1, kMmaDone = kOFree + 1, kNumBars = kMmaDone + 1;
   static constexpr int kStart = kBars + 8 * kNumBars;  // the run's first tile, TMEM base, scan scratch
-  static constexpr int kBytes = kStart + 64 + 8 * (kThreads / 32);
+  static constexpr int kBytes = kStart + 32 + 8 * (kThreads / 32);
   static constexpr uint32_t kTmemCols = N == 64 ? 512 : 256;
   static constexpr uint32_t kTmemO = 2 * kTile;
-  // the S product's A operand spans 128 rows from every chunk of Q: inside the allocation
-  static_assert(kQ + kQBufs * kQBytes - N * 128 + 128 * 128 <= kBytes, "shared memory");
+  // the S product's A operand spans 64 rows from every chunk of Q: inside the allocation
+  static_assert(kQ + kQBufs * kQBytes - N * 128 + 64 * 128 <= kBytes, "shared memory");
   static_assert(kBytes <= 227 * 1024, "shared memory");
-  static_assert(kTmemO + kPairs * N <= kTmemCols, "tensor memory");
+  static_assert(kTmemO + kMTiles * N <= kTmemCols, "tensor memory");
 };
 
 struct LatentParams {
@@ -85,7 +87,7 @@ struct LatentParams {
   const int32_t* block_table;
   int64_t bt_stride, o_tok, o_head, lse_tok;
   int num_seqs, num_tokens, num_heads, uniform_q, max_query;
-  int block_size, sub_rows, num_blocks, max_blocks;
+  int block_size, num_blocks, max_blocks;
   int group_heads, head_blocks, group_tokens;  // rows of a group = group_heads * group_tokens
   int teams, team_ctas;
   float scale_log2;
@@ -198,6 +200,81 @@ constexpr float kBias = 0.f;
 template <>
 constexpr float kBias<__half> = 7.f;
 
+// The lane that issues for a converged warp, and instructions that only it issues.
+__device__ __forceinline__ uint32_t elect_one() {
+  uint32_t e;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(e));
+  return e;
+}
+__device__ __forceinline__ void umma_elected(uint32_t tmem_d, uint64_t a, uint64_t b, uint32_t idesc,
+                                             uint32_t accumulate, uint32_t elected) {
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "setp.ne.b32 q, %5, 0;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(tmem_d),
+      "l"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(elected)
+      : "memory");
+}
+__device__ __forceinline__ void commit_elected(uint64_t* bar, uint32_t elected) {
+  asm volatile(
+      "{\n\t.reg .pred q;\n\t"
+      "setp.ne.b32 q, %1, 0;\n\t"
+      "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(smem_u32(bar)),
+      "r"(elected)
+      : "memory");
+}
+
+__device__ __forceinline__ void tma_load_5d(uint32_t dst, const CUtensorMap* map, int group, int block, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.5d.shared::cluster.global.tile.mbarrier::complete_tx::bytes "
+      "[%0], [%1, {%2, %2, %2, %3, %4}], [%5];" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(0), "r"(group), "r"(block), "r"(bar)
+      : "memory");
+}
+
+// 16 TMEM lanes x 64 columns: registers 4 i + {0, 1} hold row lane / 4, columns 8 i + 2 (lane % 4)
+// + {0, 1}; registers 4 i + {2, 3} the same columns of row lane / 4 + 8
+__device__ __forceinline__ void tmem_ld_16x64(uint32_t taddr, uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.16x256b.x8.b32 "
+      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr));
+  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+}
+
+// Barrier of the softmax warps that tells all of them whether any of them says yes.
+__device__ __forceinline__ bool softmax_any(bool v) {
+  uint32_t r;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.u32 p, %1, 0;\n\t"
+      "barrier.cta.red.or.pred q, 1, %2, p;\n\t"
+      "selp.u32 %0, 1, 0, q;\n\t}"
+      : "=r"(r)
+      : "r"(v ? 1u : 0u), "n"(kSmThreads)
+      : "memory");
+  return r != 0;
+}
+
+// Operand tiles of the KV ring: 8-token groups kGroupBytes apart, a chunk's atom 1024 bytes.
+__device__ __forceinline__ uint64_t ring_desc(uint32_t saddr) {
+  uint64_t d = 0;
+  d |= static_cast<uint64_t>((saddr & 0x3FFFFu) >> 4);
+  d |= static_cast<uint64_t>(1024 >> 4) << 16;         // next 64 columns (MN-major); unused K-major
+  d |= static_cast<uint64_t>(kGroupBytes >> 4) << 32;  // next 8 tokens
+  d |= static_cast<uint64_t>(1) << 46;
+  d |= static_cast<uint64_t>(2) << 61;
+  return d;
+}
+
 template <typename T, int N>
 __global__ void __launch_bounds__(kThreads, 1)
     latent_attention_kernel(const __grid_constant__ CUtensorMap ql_map, const __grid_constant__ CUtensorMap qr_map,
@@ -205,12 +282,12 @@ __global__ void __launch_bounds__(kThreads, 1)
   using L = Layout<N>;
   extern __shared__ __align__(1024) uint8_t smem[];
   const uint32_t sm = smem_u32(smem);
-  float* const red = reinterpret_cast<float*>(smem + L::kRed);
+  float* const row_f = reinterpret_cast<float*>(smem + L::kRowF);
+  int64_t* const row_at = reinterpret_cast<int64_t*>(smem + L::kRowAt);
   uint64_t* const bars = reinterpret_cast<uint64_t*>(smem + L::kBars);
   int* const start = reinterpret_cast<int*>(smem + L::kStart);  // b, g, t of the run's first tile
   uint32_t* const tmem_slot = reinterpret_cast<uint32_t*>(smem + L::kStart + 16);
-  int64_t* const total_slot = reinterpret_cast<int64_t*>(smem + L::kStart + 32);
-  int64_t* const scan = reinterpret_cast<int64_t*>(smem + L::kStart + 64);  // one a warp
+  int64_t* const scan = reinterpret_cast<int64_t*>(smem + L::kStart + 32);  // one a warp
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
   const int team = blockIdx.x % p.teams;
@@ -274,14 +351,12 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < L::kQBufs; ++i) mbar_init(&bars[L::kQFull + i], 1), mbar_init(&bars[L::kQEmpty + i], 1);
-    for (int i = 0; i < L::kRopeSlots; ++i) mbar_init(&bars[L::kRopeFull + i], 1), mbar_init(&bars[L::kRopeEmpty + i], 1);
-    for (int i = 0; i < L::kPairSlots; ++i) mbar_init(&bars[L::kPairFull + i], 1), mbar_init(&bars[L::kPairEmpty + i], 1);
-    for (int i = 0; i < 2; ++i) mbar_init(&bars[L::kSFull + i], 1), mbar_init(&bars[L::kSFree + i], kSmWarps);
-    mbar_init(&bars[L::kPFull], kSmWarps);
+    for (int i = 0; i < kRing; ++i) mbar_init(&bars[L::kFull + i], 1), mbar_init(&bars[L::kEmpty + i], 1);
+    for (int i = 0; i < 2; ++i) mbar_init(&bars[L::kSFull + i], 1), mbar_init(&bars[L::kSFree + i], kSmThreads / 32);
+    mbar_init(&bars[L::kPFull], kSmThreads / 32);
     mbar_init(&bars[L::kPvDone], 1);
-    mbar_init(&bars[L::kOFree], kSmWarps);
+    mbar_init(&bars[L::kOFree], kSmThreads / 32);
     mbar_init(&bars[L::kMmaDone], 2);
-    mbar_init(&bars[L::kExch], kSmWarps);
     fence_mbar_init();
   }
   if (warp == 3) {
@@ -299,378 +374,340 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   if (warp == 0) {
     // ------------------------------ TMA producer ------------------------------
-    if (lane == 0) {
+    const uint32_t elected = elect_one();
+    if (elected) {
       asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&ql_map)) : "memory");
       asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&qr_map)) : "memory");
       asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&c_map)) : "memory");
-      const int rows = p.group_heads * p.group_tokens;
-      const int sub_rows = p.sub_rows;
-      const int sub_bytes = sub_rows * 128;
-      uint32_t nq = 0, nt = 0, np = 0;  // query loads, rotary chunks and latent pairs issued
-      bool ok = true;
-      while (ok && walk.next(p, team, pc)) {
-        const int qb = nq % L::kQBufs;
-        uint64_t* const q_full = &bars[L::kQFull + qb];
-        if (nq >= L::kQBufs && !mbar_wait(&bars[L::kQEmpty + qb], (nq / L::kQBufs - 1) & 1, p.err)) break;
+    }
+    __syncwarp();
+    const int rows = p.group_heads * p.group_tokens;
+    uint32_t nq = 0, nu = 0;  // query loads and ring units so far
+    bool ok = true;
+    while (ok && walk.next(p, team, pc)) {
+      const int qb = nq % L::kQBufs;
+      uint64_t* const q_full = &bars[L::kQFull + qb];
+      if (nq >= L::kQBufs && !mbar_wait_warp(&bars[L::kQEmpty + qb], (nq / L::kQBufs - 1) & 1, p.err)) break;
+      if (elected) {
         mbar_arrive_expect_tx(q_full, kChunks * rows * 128);
         const int head = pc.g % p.head_blocks * p.group_heads;
         const int tok = pc.s.q_begin + pc.g / p.head_blocks * p.group_tokens;
         const uint32_t qdst = sm + L::kQ + qb * L::kQBytes;
-#pragma unroll 1
         for (int c = 0; c < kChunks - 1; ++c) tma_load_3d(qdst + c * N * 128, &ql_map, c * 64, head, tok, smem_u32(q_full));
         tma_load_3d(qdst + (kChunks - 1) * N * 128, &qr_map, 0, head, tok, smem_u32(q_full));
-        ++nq;
-        const int32_t* const bt = p.block_table + int64_t(pc.b) * p.bt_stride;
-        for (int t = pc.t0; t < pc.t1 && ok; ++t) {
-          const int valid = pc.valid(t);
-          if (valid <= 0) break;
-          const int subs = (valid + sub_rows - 1) / sub_rows;
-          int page[kTile / 16], row[kTile / 16];
-#pragma unroll
-          for (int i = 0; i < kTile / 16; ++i) {
-            if (i < subs) {
-              const int at = t * kTile + i * sub_rows;
-              const int lb = at / p.block_size;
-              row[i] = at - lb * p.block_size;
-              page[i] = __ldg(bt + lb);
-              if (page[i] < 0 || page[i] >= p.num_blocks) {
-                raise_device_error(p.err, NTB200_DEVERR_INDEX_RANGE);
-                page[i] = -1;  // outside the map: the rows read as zeros
-              }
-            }
-          }
-          auto load = [&](uint32_t dst, int x, uint64_t* bar) {
-#pragma unroll
-            for (int i = 0; i < kTile / 16; ++i)
-              if (i < subs) tma_load_3d(dst + i * sub_bytes, &c_map, x, row[i], page[i], smem_u32(bar));
-          };
-          const int rs = nt % L::kRopeSlots;
-          if (nt >= L::kRopeSlots && !mbar_wait(&bars[L::kRopeEmpty + rs], (nt / L::kRopeSlots - 1) & 1, p.err)) {
-            ok = false;
-            break;
-          }
-          mbar_arrive_expect_tx(&bars[L::kRopeFull + rs], subs * sub_bytes);
-          load(sm + L::kRopeRing + rs * kChunkBytes, kLatent, &bars[L::kRopeFull + rs]);
-          ++nt;
-#pragma unroll 1
-          for (int j = 0; j < kPairs; ++j) {
-            const int ps = np % L::kPairSlots;
-            if (np >= L::kPairSlots && !mbar_wait(&bars[L::kPairEmpty + ps], (np / L::kPairSlots - 1) & 1, p.err)) {
-              ok = false;
-              break;
-            }
-            mbar_arrive_expect_tx(&bars[L::kPairFull + ps], 2 * subs * sub_bytes);
-            const uint32_t dst = sm + L::kPairRing + ps * kPairBytes;
-            load(dst, j * 128, &bars[L::kPairFull + ps]);
-            load(dst + kChunkBytes, j * 128 + 64, &bars[L::kPairFull + ps]);
-            ++np;
-          }
-        }
       }
-      // drain the copies that may still be in flight
-      for (uint32_t i = nq > L::kQBufs ? nq - L::kQBufs : 0; i < nq; ++i)
-        mbar_wait(&bars[L::kQFull + i % L::kQBufs], (i / L::kQBufs) & 1, p.err);
-      for (uint32_t i = nt > L::kRopeSlots ? nt - L::kRopeSlots : 0; i < nt; ++i)
-        mbar_wait(&bars[L::kRopeFull + i % L::kRopeSlots], (i / L::kRopeSlots) & 1, p.err);
-      for (uint32_t i = np > L::kPairSlots ? np - L::kPairSlots : 0; i < np; ++i)
-        mbar_wait(&bars[L::kPairFull + i % L::kPairSlots], (i / L::kPairSlots) & 1, p.err);
-    }
-  } else if (warp == 1) {
-    // -------------------------- MMA issuer: S = Q C^T --------------------------
-    if (lane == 0) {
-      const uint32_t idesc = make_idesc(std::is_same<T, __nv_bfloat16>::value, 128, kTile);
-      uint32_t nq = 0, nt = 0, np = 0, g = 0;
-      bool ok = true;
-      while (ok && walk.next(p, team, pc)) {
-        const int qb = nq % L::kQBufs;
-        if (!mbar_wait(&bars[L::kQFull + qb], (nq / L::kQBufs) & 1, p.err)) break;
-        const uint32_t q = sm + L::kQ + qb * L::kQBytes;
-        for (int t = pc.t0; t < pc.t1 && ok; ++t, ++g) {
-          const int s = g & 1;
-          // the softmax has read this buffer's scores of two tiles ago
-          if (g >= 2 && !mbar_wait(&bars[L::kSFree + s], (g / 2 - 1) & 1, p.err)) {
-            ok = false;
-            break;
-          }
-          if (pc.valid(t) > 0) {
-            const int rs = nt % L::kRopeSlots;
-            if (!mbar_wait(&bars[L::kRopeFull + rs], (nt / L::kRopeSlots) & 1, p.err)) {
-              ok = false;
-              break;
-            }
-            tc_fence_after();
-            const uint64_t ar = sw128_kmajor_desc(q + (kChunks - 1) * N * 128);
-            const uint64_t br = sw128_kmajor_desc(sm + L::kRopeRing + rs * kChunkBytes);
-#pragma unroll
-            for (int k = 0; k < 4; ++k) umma_f16(tmem + s * kTile, ar + 2 * k, br + 2 * k, idesc, k ? 1u : 0u);
-            umma_commit(&bars[L::kRopeEmpty + rs]);
-            ++nt;
-#pragma unroll 1
-            for (int j = 0; j < kPairs; ++j, ++np) {
-              const int ps = np % L::kPairSlots;
-              if (!mbar_wait(&bars[L::kPairFull + ps], (np / L::kPairSlots) & 1, p.err)) {
-                ok = false;
-                break;
-              }
-              tc_fence_after();
-#pragma unroll
-              for (int h = 0; h < 2; ++h) {
-                const uint64_t a = sw128_kmajor_desc(q + (2 * j + h) * N * 128);
-                const uint64_t b = sw128_kmajor_desc(sm + L::kPairRing + ps * kPairBytes + h * kChunkBytes);
-#pragma unroll
-                for (int k = 0; k < 4; ++k) umma_f16(tmem + s * kTile, a + 2 * k, b + 2 * k, idesc, 1u);
-              }
-            }
-          }
-          umma_commit(&bars[L::kSFull + s]);
-        }
-        umma_commit(&bars[L::kQEmpty + qb]);
-        ++nq;
-      }
-      // every issued MMA completes before TMEM may be released
-      umma_commit(&bars[L::kMmaDone]);
-      mbar_wait(&bars[L::kMmaDone], 0, p.err);
-    }
-  } else if (warp == 2) {
-    // ------------------------ MMA issuer: O^T += C^T P^T ------------------------
-    if (lane == 0) {
-      const uint32_t idesc = make_idesc(std::is_same<T, __nv_bfloat16>::value, 128, N) | (1u << 15);  // A MN-major
-      uint32_t np = 0, g = 0, pieces = 0;
-      bool ok = true;
-      while (ok && walk.next(p, team, pc)) {
-        for (int t = pc.t0; t < pc.t1 && ok; ++t, ++g) {
-          // the first product of a piece overwrites O^T: the one before has been written out
-          if (!mbar_wait(&bars[L::kPFull], g & 1, p.err) ||
-              (t == pc.t0 && pieces >= 1 && !mbar_wait(&bars[L::kOFree], (pieces - 1) & 1, p.err))) {
-            ok = false;
-            break;
-          }
-          const int valid = pc.valid(t);
-          if (valid > 0) {
-            const int ks = (valid + 15) / 16;
-            tc_fence_after();
-            const uint64_t b = sw128_kmajor_desc(sm + L::kP);
-#pragma unroll 1
-            for (int j = 0; j < kPairs; ++j, ++np) {
-              const int ps = np % L::kPairSlots;
-              const uint32_t base = sm + L::kPairRing + ps * kPairBytes;
-              for (int k = 0; k < ks; ++k)
-                umma_f16(tmem + L::kTmemO + j * N, sw128_mnmajor_desc(base + k * 2048, kChunkBytes), b + 2 * k, idesc,
-                         (t > pc.t0 || k > 0) ? 1u : 0u);
-              umma_commit(&bars[L::kPairEmpty + ps]);
-            }
-          }
-          umma_commit(&bars[L::kPvDone]);
-        }
-        ++pieces;
-      }
-      umma_commit(&bars[L::kMmaDone]);
-      mbar_wait(&bars[L::kMmaDone], 0, p.err);
-    }
-  } else if (warp >= kFirstSmWarp) {
-    // ------------------------------ softmax + output ------------------------------
-    // Warp (quad, part): scores of rows 32 quad + lane at tokens 16 part .. + 16 (when the group
-    // has such rows), and the block of O^T at latent columns 128 part + 32 quad + lane.  Every
-    // warp holds the running max of all rows (lane's and lane + 32's), so all agree on when to
-    // rescale without another exchange.
-    constexpr int kRowRegs = N == 64 ? 2 : 1;
-    const int quad = warp & 3;
-    const int part = (warp - kFirstSmWarp) >> 2;
-    const int r = quad * 32 + lane;
-    const bool active = quad * 32 < N;
-    const uint32_t lanes = uint32_t(quad * 32) << 16;
-    const uint32_t o_tmem = tmem + L::kTmemO + part * N + lanes;
-    uint64_t* const exch = &bars[L::kExch];
-    uint32_t uses = 0;
-    // Publishes an active thread's value for its row and leaves every row's four in `red`.
-    auto exchange = [&](float v) -> const float* {
-      float* const buf = red + (uses & 1) * (kParts * kMaxRows);
-      if (active) buf[part * kMaxRows + r] = v;
       __syncwarp();
-      if (lane == 0) mbar_arrive(exch);
-      const bool got = mbar_wait_warp(exch, uses & 1, p.err);
-      ++uses;
-      return got ? buf : nullptr;
-    };
-    uint32_t g = 0, np = 0, pieces = 0;
-    bool ok = true;
-    while (ok && walk.next(p, team, pc)) {
-      const int tok0 = pc.g / p.head_blocks * p.group_tokens;
-      const int head0 = pc.g % p.head_blocks * p.group_heads;
-      // rows of the group: (token, head) = (row / group_heads, row % group_heads)
-      auto row_there = [&](int row, int& tok, int& head) {
-        const int rt = row / p.group_heads;
-        tok = tok0 + rt;
-        head = head0 + row - rt * p.group_heads;
-        return rt < p.group_tokens && tok < pc.s.q_len && head < p.num_heads;
+      ++nq;
+      const int32_t* const bt = p.block_table + int64_t(pc.b) * p.bt_stride;
+      const int first = pc.t0 * kTileUnits;
+      const int last = (min(pc.keys, pc.t1 * kTile) + kUnit - 1) / kUnit;  // units [first, last) hold keys
+      // 32 units' page ids and groups at a time, one a lane, the next 32 fetched ahead
+      int page = -1, group = 0, next_page = -1, next_group = 0;
+      auto fetch = [&](int base) {
+        const int tok = (base + lane) * kUnit;
+        const int lb = tok / p.block_size;
+        next_group = (tok - lb * p.block_size) / 8;
+        next_page = base + lane < last ? __ldg(bt + lb) : 0;
       };
-      int tok, head;
-      const bool there = row_there(r, tok, head);
-      // this row sees keys [0, limit)
-      const int limit = there && active ? max(pc.s.ctx - pc.s.q_len + tok + 1, 0) : 0;
-      float m[kRowRegs];
-#pragma unroll
-      for (int i = 0; i < kRowRegs; ++i) m[i] = -INFINITY;
-      float l_run = 0.f;
-      for (int t = pc.t0; t < pc.t1; ++t, ++g) {
-        const int s = g & 1;
-        const int valid = pc.valid(t);
-        if (!mbar_wait_warp(&bars[L::kSFull + s], (g / 2) & 1, p.err)) {
+      fetch(first);
+      // a tile is always four units of the ring, those past the last key empty
+      const int end = (last + kTileUnits - 1) / kTileUnits * kTileUnits;
+      for (int u = first; ok && u < end; ++u, ++nu) {
+        const int i = (u - first) & 31;
+        if (i == 0) {
+          page = next_page;
+          group = next_group;
+          if (page < 0 || page >= p.num_blocks) {
+            raise_device_error(p.err, NTB200_DEVERR_INDEX_RANGE);
+            page = -1;  // outside the map: the rows read as zeros
+          }
+          if (u + 32 < last) fetch(u + 32);
+        }
+        const int at_page = __shfl_sync(0xffffffffu, page, i);
+        const int at_group = __shfl_sync(0xffffffffu, group, i);
+        const uint32_t s = nu % kRing;
+        if (nu >= kRing && !mbar_wait_warp(&bars[L::kEmpty + s], (nu / kRing - 1) & 1, p.err)) {
           ok = false;
           break;
         }
-        tc_fence_after();
-        float x[kPartCols];
-        float mx = -INFINITY;
-        if (active) {
-          uint32_t v[kPartCols];
-          __syncwarp();
-          tmem_ld_16(tmem + lanes + s * kTile + part * kPartCols, v);
-          const int seen = limit - t * kTile - part * kPartCols;
+        if (elected) {
+          if (u < last) {
+            mbar_arrive_expect_tx(&bars[L::kFull + s], kUnitBytes);
+            tma_load_5d(sm + L::kKv + s * kUnitBytes, &c_map, at_group, at_page, smem_u32(&bars[L::kFull + s]));
+          } else {
+            mbar_arrive(&bars[L::kFull + s]);
+          }
+        }
+        __syncwarp();
+      }
+    }
+    // drain the copies that may still be in flight
+    for (uint32_t i = nq > L::kQBufs ? nq - L::kQBufs : 0; i < nq; ++i)
+      mbar_wait_warp(&bars[L::kQFull + i % L::kQBufs], (i / L::kQBufs) & 1, p.err);
+    for (uint32_t i = nu > kRing ? nu - kRing : 0; i < nu; ++i)
+      mbar_wait_warp(&bars[L::kFull + i % kRing], (i / kRing) & 1, p.err);
+  } else if (warp == 1) {
+    // -------------------------- MMA issuer: S = Q C^T --------------------------
+    const uint32_t elected = elect_one();
+    const uint32_t idesc = make_idesc(std::is_same<T, __nv_bfloat16>::value, 64, kTile);
+    uint32_t nq = 0, nu = 0, g = 0;
+    bool ok = true;
+    while (ok && walk.next(p, team, pc)) {
+      const int qb = nq % L::kQBufs;
+      if (!mbar_wait_warp(&bars[L::kQFull + qb], (nq / L::kQBufs) & 1, p.err)) break;
+      const uint64_t a0 = sw128_kmajor_desc(sm + L::kQ + qb * L::kQBytes);
+      for (int t = pc.t0; t < pc.t1; ++t, ++g) {
+        const int s = g & 1;
+        // the softmax has read this buffer's scores of two tiles ago
+        if (g >= 2) ok = mbar_wait_warp(&bars[L::kSFree + s], (g / 2 - 1) & 1, p.err);
+        if (pc.valid(t) > 0) {
+          for (int i = 0; i < kTileUnits && ok; ++i)
+            ok = mbar_wait_warp(&bars[L::kFull + (nu + i) % kRing], ((nu + i) / kRing) & 1, p.err);
+          if (!ok) break;
+          tc_fence_after();
+          const uint64_t b0 = ring_desc(sm + L::kKv + nu % kRing * kUnitBytes);
 #pragma unroll
-          for (int i = 0; i < kPartCols; ++i) {
-            x[i] = i < seen ? __uint_as_float(v[i]) * p.scale_log2 : -INFINITY;
-            mx = fmaxf(mx, x[i]);
+          for (int c = 0; c < kChunks; ++c)
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              umma_elected(tmem + s * kTile, a0 + c * (N * 128 >> 4) + 2 * k, b0 + c * (1024 >> 4) + 2 * k, idesc,
+                           (c | k) ? 1u : 0u, elected);
+          nu += kTileUnits;
+        }
+        if (!ok) break;
+        commit_elected(&bars[L::kSFull + s], elected);
+      }
+      commit_elected(&bars[L::kQEmpty + qb], elected);
+      ++nq;
+    }
+    // every issued MMA completes before TMEM may be released
+    commit_elected(&bars[L::kMmaDone], elected);
+    mbar_wait_warp(&bars[L::kMmaDone], 0, p.err);
+  } else if (warp == 2) {
+    // ------------------------ MMA issuer: O^T += C^T P^T ------------------------
+    const uint32_t elected = elect_one();
+    const uint32_t idesc = make_idesc(std::is_same<T, __nv_bfloat16>::value, 128, N) | (1u << 15);  // A MN-major
+    const uint64_t b0 = sw128_kmajor_desc(sm + L::kP);
+    uint32_t nu = 0, g = 0, pieces = 0;
+    bool ok = true;
+    while (ok && walk.next(p, team, pc)) {
+      for (int t = pc.t0; t < pc.t1; ++t, ++g) {
+        // the first product of a piece overwrites O^T: the one before has been written out
+        ok = mbar_wait_warp(&bars[L::kPFull], g & 1, p.err) &&
+             (t > pc.t0 || pieces == 0 || mbar_wait_warp(&bars[L::kOFree], (pieces - 1) & 1, p.err));
+        if (!ok) break;
+        const int valid = pc.valid(t);
+        if (valid > 0) {
+          tc_fence_after();
+          const int steps = (valid + kUnit - 1) / kUnit;
+          const uint64_t a0 = ring_desc(sm + L::kKv + nu % kRing * kUnitBytes);
+#pragma unroll
+          for (int k = 0; k < kTileUnits; ++k) {
+            if (k < steps) {
+#pragma unroll
+              for (int j = 0; j < kMTiles; ++j)
+                umma_elected(tmem + L::kTmemO + j * N, a0 + k * (kUnitBytes >> 4) + j * (2048 >> 4), b0 + 2 * k, idesc,
+                             (t > pc.t0 || k > 0) ? 1u : 0u, elected);
+            }
+            commit_elected(&bars[L::kEmpty + (nu + k) % kRing], elected);
+          }
+          nu += kTileUnits;
+        }
+        commit_elected(&bars[L::kPvDone], elected);
+      }
+      ++pieces;
+    }
+    commit_elected(&bars[L::kMmaDone], elected);
+    mbar_wait_warp(&bars[L::kMmaDone], 0, p.err);
+  } else if (warp >= kFirstSmWarp) {
+    // ------------------------------ softmax + output ------------------------------
+    // The M = 64 product leaves row r in TMEM lane 32 (r / 16) + r % 16: warp `quad` has rows
+    // 16 quad .. + 16, this lane the columns 8 i + 2 (lane % 4) + {0, 1} of rows r0 and r0 + 8.  O^T
+    // covers all lanes: every warp rescales and writes its 32 latent columns of each M tile.
+    // A wait that gave up is told to the other warps at the next barrier, where all leave.
+    const int quad = warp & 3;
+    const bool active = quad * 16 < N;
+    const int r0 = quad * 16 + (lane >> 2);
+    const uint32_t lanes = uint32_t(quad * 32) << 16;
+    const uint32_t o_tmem = tmem + L::kTmemO + lanes;
+    const int col0 = 2 * (lane & 3);
+    uint32_t g = 0, nu = 0, pieces = 0;
+    bool bad = false;
+    while (!bad && walk.next(p, team, pc)) {
+      const int tok0 = pc.g / p.head_blocks * p.group_tokens;
+      const int head0 = pc.g % p.head_blocks * p.group_heads;
+      // rows of the group: (token, head) = (row / group_heads, row % group_heads); this lane's two
+      int tok[2], head[2], limit[2];
+      bool there[2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int row = r0 + 8 * i;
+        const int rt = row / p.group_heads;
+        tok[i] = tok0 + rt;
+        head[i] = head0 + row - rt * p.group_heads;
+        there[i] = active && rt < p.group_tokens && tok[i] < pc.s.q_len && head[i] < p.num_heads;
+        limit[i] = there[i] ? max(pc.s.ctx - pc.s.q_len + tok[i] + 1, 0) : 0;  // sees keys [0, limit)
+      }
+      float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+      bool left = false;
+      for (int t = pc.t0; t < pc.t1; ++t, ++g) {
+        const int s = g & 1;
+        const int valid = pc.valid(t);
+        bad = bad || !mbar_wait_warp(&bars[L::kSFull + s], (g / 2) & 1, p.err);
+        tc_fence_after();
+        float x[32];
+        float alpha[2] = {1.f, 1.f};
+        bool grow = false;
+        if (active) {
+          {
+            uint32_t v[32];
+            __syncwarp();
+            tmem_ld_16x64(tmem + lanes + s * kTile, v);
+#pragma unroll
+            for (int i = 0; i < 32; ++i) x[i] = __uint_as_float(v[i]) * p.scale_log2;
+          }
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const int seen = limit[h] - t * kTile - col0;
+            if (seen < kTile - col0) {
+#pragma unroll
+              for (int i = 0; i < 8; ++i)
+#pragma unroll
+                for (int e = 0; e < 2; ++e)
+                  if (8 * i + e >= seen) x[4 * i + 2 * h + e] = -INFINITY;
+            }
+            float mx = -INFINITY;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) mx = fmaxf(mx, fmaxf(x[4 * i + 2 * h], x[4 * i + 2 * h + 1]));
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+            const float m_new = fmaxf(m[h], mx);
+            if (m_new > m[h] + kRescaleLog2) {  // also true for the first finite maximum
+              alpha[h] = hw_exp2(m[h] - m_new);
+              m[h] = m_new;
+              l[h] *= alpha[h];
+              grow = true;
+            }
           }
         }
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&bars[L::kSFree + s]);
-        const float* const all = exchange(mx);
-        if (all == nullptr) {
-          ok = false;
-          break;
+        const bool news = softmax_any(grow || bad);
+        if (news) {
+          if ((lane & 3) == 0 && active) row_f[r0] = alpha[0], row_f[r0 + 8] = alpha[1];
+          left = softmax_any(bad);
+          if (left) break;
         }
-        float alpha[kRowRegs];
-        bool grow = false;
-#pragma unroll
-        for (int i = 0; i < kRowRegs; ++i) {
-          const int row = lane + 32 * i;
-          float m_new = m[i];
-#pragma unroll
-          for (int q = 0; q < kParts; ++q)
-            if (row < N) m_new = fmaxf(m_new, all[q * kMaxRows + row]);
-          const bool up = m_new > m[i] + kRescaleLog2;  // also true for the first finite max
-          alpha[i] = up ? hw_exp2(m[i] - m_new) : 1.f;
-          if (up) m[i] = m_new;
-          grow = grow || up;
-        }
-        const bool any = __any_sync(0xffffffffu, grow);
-        uint32_t pk[kPartCols / 2];
+        uint32_t pk[16];
         if (active) {
-          const float mine_m = kRowRegs == 2 && quad == 1 ? m[kRowRegs - 1] : m[0];
-          const float mine_a = kRowRegs == 2 && quad == 1 ? alpha[kRowRegs - 1] : alpha[0];
-          const float m_use = mine_m == -INFINITY ? 0.f : mine_m - kBias<T>;
-          l_run *= mine_a;
-          float l2[2] = {0.f, 0.f};
 #pragma unroll
-          for (int i = 0; i < kPartCols / 2; ++i) {
-            const float p0 = hw_exp2(x[2 * i] - m_use);
-            const float p1 = hw_exp2(x[2 * i + 1] - m_use);
-            l2[i & 1] += p0 + p1;
-            Pair<T>::store(reinterpret_cast<T*>(&pk[i]), p0, p1);
+          for (int h = 0; h < 2; ++h) {
+            const float m_use = m[h] == -INFINITY ? 0.f : m[h] - kBias<T>;
+            float sum = 0.f;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              const float p0 = hw_exp2(x[4 * i + 2 * h] - m_use);
+              const float p1 = hw_exp2(x[4 * i + 2 * h + 1] - m_use);
+              sum += p0 + p1;
+              Pair<T>::store(reinterpret_cast<T*>(&pk[2 * i + h]), p0, p1);
+            }
+            l[h] += sum;
           }
-          l_run += l2[0] + l2[1];
         }
         // P and O^T are free once the product of the tile before is complete
-        if (g >= 1 && !mbar_wait_warp(&bars[L::kPvDone], (g - 1) & 1, p.err)) {
-          ok = false;
-          break;
-        }
-        if (any && t > pc.t0) {
+        if (g >= 1) bad = bad || !mbar_wait_warp(&bars[L::kPvDone], (g - 1) & 1, p.err);
+        if (news && t > pc.t0) {
           tc_fence_after();
+#pragma unroll 1
+          for (int j = 0; j < kMTiles; ++j)
+#pragma unroll 1
+            for (int c0 = 0; c0 < N; c0 += 16) {
+              uint32_t v[16];
+              __syncwarp();
+              tmem_ld_16(o_tmem + j * N + c0, v);
 #pragma unroll
-          for (int c0 = 0; c0 < N; c0 += 16) {
-            uint32_t v[16];
-            __syncwarp();
-            tmem_ld_16(o_tmem + c0, v);
-#pragma unroll
-            for (int c = 0; c < 16; ++c) {
-              const float a = __shfl_sync(0xffffffffu, alpha[(c0 + c) / 32], (c0 + c) % 32);
-              v[c] = __float_as_uint(__uint_as_float(v[c]) * a);
+              for (int c = 0; c < 16; ++c) v[c] = __float_as_uint(__uint_as_float(v[c]) * row_f[c0 + c]);
+              tmem_st_16(o_tmem + j * N + c0, v);
             }
-            tmem_st_16(o_tmem + c0, v);
-          }
           asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
         }
-        if (active && r < N) {
-          // P [row, token], 128-byte swizzled rows; this part's 16 tokens are two 16-byte units
-          uint8_t* const prow = smem + L::kP + r * 128;
+        if (active) {
+          // P [row, token], 128-byte swizzled rows: 8 tokens a 16-byte unit, two a lane
 #pragma unroll
-          for (int i = 0; i < 2; ++i)
-            *reinterpret_cast<uint4*>(prow + (((part * 2 + i) ^ (r & 7)) << 4)) =
-                make_uint4(pk[4 * i], pk[4 * i + 1], pk[4 * i + 2], pk[4 * i + 3]);
+          for (int h = 0; h < 2; ++h) {
+            const int row = r0 + 8 * h;
+            uint8_t* const prow = smem + L::kP + row * 128 + (lane & 3) * 4;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) *reinterpret_cast<uint32_t*>(prow + ((i ^ (row & 7)) << 4)) = pk[2 * i + h];
+          }
         }
         if (valid > 0) {
           if (valid & 15) {
             // rows past the last visible key, up to the product's next step of 16, hold whatever
             // memory held there: zeroed, so that P = 0 never meets a non-finite value
-            const int t0 = valid, n = 16 - (valid & 15);
-            for (int i = threadIdx.x - 32 * kFirstSmWarp; i < n * 64; i += 32 * kSmWarps) {
-              const int c = (i >> 3) & 7;  // chunk
-              const uint32_t ps = (np + (c >> 1)) % L::kPairSlots;
-              *reinterpret_cast<uint4*>(smem + L::kPairRing + ps * kPairBytes + (c & 1) * kChunkBytes +
-                                        (t0 + (i >> 6)) * 128 + (i & 7) * 16) = make_uint4(0u, 0u, 0u, 0u);
+            const int n = 16 - (valid & 15);
+            uint8_t* const tile = smem + L::kKv + nu % kRing * kUnitBytes;
+            for (int i = threadIdx.x - 32 * kFirstSmWarp; i < n * 64; i += kSmThreads) {
+              const int row = valid + (i >> 6);
+              *reinterpret_cast<uint4*>(tile + (row >> 3) * kGroupBytes + ((i >> 3) & 7) * 1024 + (row & 7) * 128 +
+                                        (i & 7) * 16) = make_uint4(0u, 0u, 0u, 0u);
             }
           }
-          np += kPairs;
+          nu += kTileUnits;
         }
         fence_proxy_async_smem();  // P and the zeros -> tensor core
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&bars[L::kPFull]);
       }
-      if (!ok) break;
+      if (left) break;
       // O^T is final once the piece's last product is complete
-      ok = mbar_wait_warp(&bars[L::kPvDone], (g - 1) & 1, p.err);
-      const float* const all = ok ? exchange(l_run) : nullptr;
-      if (all == nullptr) {
-        ok = false;
-        break;
-      }
-      tc_fence_after();
+      bad = bad || !mbar_wait_warp(&bars[L::kPvDone], (g - 1) & 1, p.err);
       const bool whole = pc.t0 == 0 && pc.t1 == pc.n;
       const int64_t share = int64_t(blockIdx.x) * 2 + (pieces > 0 ? 1 : 0);
-      float inv[kRowRegs];
-      int64_t dst[kRowRegs];  // element offset of the row's output, -1: no such row
 #pragma unroll
-      for (int i = 0; i < kRowRegs; ++i) {
-        const int row = lane + 32 * i;
-        float l = 0.f;
-        if (row < N)
-#pragma unroll
-          for (int q = 0; q < kParts; ++q) l += all[q * kMaxRows + row];
-        inv[i] = l == 0.f ? 0.f : 1.f / l;
-        int rtok, rhead;
-        const bool rthere = row_there(row, rtok, rhead) && row < N;
-        const float lse2 = l == 0.f ? -INFINITY : m[i] - kBias<T> + log2f(l);
-        if (whole) {
-          dst[i] = rthere ? int64_t(pc.s.q_begin + rtok) * p.o_tok + int64_t(rhead) * p.o_head : -1;
-          if (rthere && p.lse != nullptr && quad == 0 && part == 0)
-            p.lse[int64_t(pc.s.q_begin + rtok) * p.lse_tok + rhead] = lse2 * 0.6931471805599453f;
-        } else {
-          dst[i] = rthere ? (share * kMaxRows + row) * kLatent : -1;
-          if (rthere && quad == 0 && part == 0) p.part_lse[share * kMaxRows + row] = lse2;
+      for (int h = 0; h < 2; ++h) {
+        const int row = r0 + 8 * h;
+        float sum = l[h];
+        sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+        sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+        if (active && (lane & 3) == 0) {
+          const float lse2 = sum == 0.f ? -INFINITY : m[h] - kBias<T> + log2f(sum);
+          row_f[row] = sum == 0.f ? 0.f : 1.f / sum;
+          if (whole) {
+            const int64_t at = int64_t(pc.s.q_begin + tok[h]);
+            row_at[row] = there[h] ? at * p.o_tok + int64_t(head[h]) * p.o_head : -1;
+            if (there[h] && p.lse != nullptr) p.lse[at * p.lse_tok + head[h]] = lse2 * 0.6931471805599453f;
+          } else {
+            row_at[row] = there[h] ? (share * kMaxRows + row) * kLatent : -1;
+            if (there[h]) p.part_lse[share * kMaxRows + row] = lse2;
+          }
         }
       }
-      if (!whole && quad == 0 && part == 0 && lane == 0) {
+      if (!whole && warp == kFirstSmWarp && lane == 0) {
         p.desc[share * 2] = make_int4(1, pc.t0, pc.t1, pc.n);
-        p.desc[share * 2 + 1] = make_int4(pc.s.q_begin + tok0, pc.s.q_len - tok0, head0, 0);
+        p.desc[share * 2 + 1] = make_int4(pc.s.q_begin + tok0, pc.s.q_len - tok0, head0, int(min(per, int64_t(0x7fffffff))));
       }
-      const int col = part * 128 + quad * 32 + lane;
+      if (softmax_any(bad)) break;
+      tc_fence_after();
+#pragma unroll 1
+      for (int j = 0; j < kMTiles; ++j) {
+        const int col = j * 128 + quad * 32 + lane;
+#pragma unroll 1
+        for (int c0 = 0; c0 < N; c0 += 16) {
+          uint32_t v[16];
+          __syncwarp();
+          tmem_ld_16(o_tmem + j * N + c0, v);
 #pragma unroll
-      for (int c0 = 0; c0 < N; c0 += 16) {
-        uint32_t v[16];
-        __syncwarp();
-        tmem_ld_16(o_tmem + c0, v);
-#pragma unroll
-        for (int c = 0; c < 16; ++c) {
-          const float k = __shfl_sync(0xffffffffu, inv[(c0 + c) / 32], (c0 + c) % 32);
-          const int64_t at = __shfl_sync(0xffffffffu, dst[(c0 + c) / 32], (c0 + c) % 32);
-          if (at < 0) continue;
-          const float o = k == 0.f ? 0.f : __uint_as_float(v[c]) * k;  // an empty row's O^T was never written
-          if (whole) static_cast<T*>(p.out)[at + col] = Elem<T>::from_f(o);
-          else p.part_o[at + col] = o;
+          for (int c = 0; c < 16; ++c) {
+            const float k = row_f[c0 + c];
+            const int64_t at = row_at[c0 + c];
+            if (at < 0) continue;
+            const float o = k == 0.f ? 0.f : __uint_as_float(v[c]) * k;  // an empty row's O^T was never written
+            if (whole) static_cast<T*>(p.out)[at + col] = Elem<T>::from_f(o);
+            else p.part_o[at + col] = o;
+          }
         }
       }
       tc_fence_before();
@@ -689,57 +726,65 @@ __global__ void __launch_bounds__(kThreads, 1)
 }
 
 // Joins the shares of every item that was cut.  The CTA whose first piece ends an item (its
-// share 0 has t0 > 0 and t1 = n) names that item; the shares before it are the last ones of
-// the CTAs before, back to the one that starts at tile 0.
-constexpr int kJoinThreads = kLatent / 4;
-constexpr int kJoinRows = 4;  // rows a CTA
+// share 0 has t0 > 0 and t1 = n) names that item.  Every CTA between the item's first and this one
+// had nothing else to do, so their number follows from t0 and the tiles a CTA.  A thread sums
+// four columns of a row over every fourth share; the four sums meet in shared memory.
+constexpr int kJoinCols = kLatent / 4;
+constexpr int kJoinParts = 4;
+constexpr int kJoinRows = 2;  // rows a CTA
 
 template <typename T>
-__global__ void __launch_bounds__(kJoinThreads) latent_join_kernel(const LatentParams p) {
-  __shared__ int list[1024];  // shares of the item
+__global__ void __launch_bounds__(kJoinCols * kJoinParts) latent_join_kernel(const LatentParams p) {
+  __shared__ float4 sums[kJoinParts][kJoinCols];
+  __shared__ float weights[kJoinParts];
+  const int part = threadIdx.x / kJoinCols, col = threadIdx.x % kJoinCols;
   pdl_trigger();
   pdl_wait();
   const int cta = blockIdx.x;
   const int4 end = p.desc[int64_t(cta) * 4];
   if (end.x == 0 || end.y == 0 || end.z != end.w) return;
   const int4 where = p.desc[int64_t(cta) * 4 + 1];
-  __shared__ int num;
-  if (threadIdx.x == 0) {
-    int n = 0;
-    list[n++] = cta * 2;
-    for (int c = cta - p.teams; c >= 0 && n < 1024; c -= p.teams) {
-      const int share = c * 2 + (p.desc[int64_t(c) * 4 + 2].x != 0 ? 1 : 0);
-      list[n++] = share;
-      if (p.desc[int64_t(share) * 2].y == 0) break;
-    }
-    num = n;
-  }
-  __syncthreads();
-  const int n = num;
+  const int n = 1 + (end.y + where.w - 1) / where.w;
+  const int first = cta - (n - 1) * p.teams;
+  const int first_share = first * 2 + (p.desc[int64_t(first) * 4 + 2].x != 0 ? 1 : 0);
+  auto share = [&](int i) { return int64_t(i == 0 ? first_share : 2 * (first + i * p.teams)); };
   for (int r = blockIdx.y * kJoinRows; r < (int(blockIdx.y) + 1) * kJoinRows; ++r) {
     const int tok = r / p.group_heads;
     const int head = where.z + r - tok * p.group_heads;
     if (tok >= p.group_tokens || tok >= where.y || head >= p.num_heads) continue;
     float top = -INFINITY;
-    for (int i = 0; i < n; ++i) top = fmaxf(top, p.part_lse[int64_t(list[i]) * kMaxRows + r]);
+#pragma unroll 8
+    for (int i = 0; i < n; ++i) top = fmaxf(top, p.part_lse[share(i) * kMaxRows + r]);
     const float ref = top == -INFINITY ? 0.f : top;
     float sum = 0.f;
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-    for (int i = 0; i < n; ++i) {
-      const int64_t row = int64_t(list[i]) * kMaxRows + r;
+#pragma unroll 8
+    for (int i = part; i < n; i += kJoinParts) {
+      const int64_t row = share(i) * kMaxRows + r;
       const float w = exp2f(p.part_lse[row] - ref);
-      const float4 o = reinterpret_cast<const float4*>(p.part_o + row * kLatent)[threadIdx.x];
+      const float4 o = reinterpret_cast<const float4*>(p.part_o + row * kLatent)[col];
       sum += w;
       acc.x += w * o.x, acc.y += w * o.y, acc.z += w * o.z, acc.w += w * o.w;
     }
-    const float inv = sum == 0.f ? 0.f : 1.f / sum;
-    const float y[4] = {acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv};
-    T* const o = static_cast<T*>(p.out) + int64_t(where.x + tok) * p.o_tok + int64_t(head) * p.o_head;
-    *reinterpret_cast<Vec<T, 4>*>(o + threadIdx.x * 4) = pack_f<T, 4>(y);
-    if (p.lse != nullptr && threadIdx.x == 0)
-      p.lse[int64_t(where.x + tok) * p.lse_tok + head] =
-          sum == 0.f ? -INFINITY : (ref + log2f(sum)) * 0.6931471805599453f;
+    sums[part][col] = acc;
+    if (col == 0) weights[part] = sum;
+    __syncthreads();
+    if (part == 0) {
+#pragma unroll
+      for (int q = 1; q < kJoinParts; ++q) {
+        const float4 o = sums[q][col];
+        sum += weights[q];
+        acc.x += o.x, acc.y += o.y, acc.z += o.z, acc.w += o.w;
+      }
+      const float inv = sum == 0.f ? 0.f : 1.f / sum;
+      const float y[4] = {acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv};
+      T* const o = static_cast<T*>(p.out) + int64_t(where.x + tok) * p.o_tok + int64_t(head) * p.o_head;
+      *reinterpret_cast<Vec<T, 4>*>(o + col * 4) = pack_f<T, 4>(y);
+      if (p.lse != nullptr && col == 0)
+        p.lse[int64_t(where.x + tok) * p.lse_tok + head] =
+            sum == 0.f ? -INFINITY : (ref + log2f(sum)) * 0.6931471805599453f;
+    }
+    __syncthreads();
   }
 }
 
@@ -761,17 +806,18 @@ int make_query_map(CUtensorMap* map, const void* base, bool bf16, int64_t dim, i
   return NTB200_OK;
 }
 
-// the cache [blocks, block_size, 576]: box = sub_rows tokens of a page x 64 columns
+// the cache [blocks, block_size, 576] as (64 columns, 8 tokens, 9 chunks, groups of 8 tokens,
+// blocks): box = 16 tokens' whole rows, laid down group by group, chunk by chunk
 int make_cache_map(CUtensorMap* map, const void* base, bool bf16, int64_t blocks, int64_t block_size,
-                   int64_t block_stride, int64_t page_stride, int sub_rows) {
+                   int64_t block_stride, int64_t page_stride) {
   EncodeTiledFn enc = encode_fn();
   if (enc == nullptr) return fail(NTB200_ERR_CUDA, "cuTensorMapEncodeTiled unavailable");
-  const cuuint64_t dims[3] = {cuuint64_t(kLatent + kRope), cuuint64_t(block_size), cuuint64_t(blocks)};
-  const cuuint64_t strides[2] = {cuuint64_t(page_stride * 2),
+  const cuuint64_t dims[5] = {64, 8, cuuint64_t(kChunks), cuuint64_t(block_size / 8), cuuint64_t(blocks)};
+  const cuuint64_t strides[4] = {cuuint64_t(page_stride * 2), 128, cuuint64_t(page_stride * 16),
                                  cuuint64_t((blocks > 1 ? block_stride : block_size * page_stride) * 2)};
-  const cuuint32_t box[3] = {64, cuuint32_t(sub_rows), 1};
-  const cuuint32_t estr[3] = {1, 1, 1};
-  const CUresult r = enc(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3,
+  const cuuint32_t box[5] = {64, 8, cuuint32_t(kChunks), kUnit / 8, 1};
+  const cuuint32_t estr[5] = {1, 1, 1, 1, 1};
+  const CUresult r = enc(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 5,
                          const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
                          CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                          CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
@@ -790,7 +836,7 @@ int launch_latent(const CUtensorMap& ql, const CUtensorMap& qr, const CUtensorMa
   if (st != NTB200_OK || p.team_ctas == 1) return st;  // one CTA a team cuts no item
   const int rows = p.group_heads * p.group_tokens;
   return launch_kernel("latent_attention (join)", latent_join_kernel<T>,
-                       dim3(ctas, unsigned(ceil_div(rows, kJoinRows))), dim3(kJoinThreads), 0, s, p);
+                       dim3(ctas, unsigned(ceil_div(rows, kJoinRows))), dim3(kJoinCols * kJoinParts), 0, s, p);
 }
 
 template <typename T>
@@ -869,7 +915,6 @@ extern "C" int ntb200_latent_attention(
   p.uniform_q = query_start_loc == nullptr ? int(num_tokens / num_seqs) : 0;
   p.max_query = query_start_loc == nullptr ? p.uniform_q : int(std::min<int64_t>(max_query_len, num_tokens));
   p.block_size = int(block_size);
-  p.sub_rows = block_size % 64 == 0 ? 64 : block_size % 32 == 0 ? 32 : 16;
   p.num_blocks = int(num_blocks);
   p.max_blocks = int(max_blocks_per_seq);
   p.head_blocks = int(ceil_div(num_heads, kMaxRows));
@@ -897,7 +942,7 @@ extern "C" int ntb200_latent_attention(
                       p.group_heads);
   if (st != NTB200_OK) return st;
   if (max_blocks_per_seq > 0) {
-    st = make_cache_map(&c, kv_cache, bf16, num_blocks, block_size, cache_block_stride, cache_page_stride, p.sub_rows);
+    st = make_cache_map(&c, kv_cache, bf16, num_blocks, block_size, cache_block_stride, cache_page_stride);
     if (st != NTB200_OK) return st;
   } else {
     c = ql;  // never read: every context is empty
