@@ -74,7 +74,7 @@ def test_store(change, status):
 
 @pytest.mark.parametrize("change,status", [
     ({31: 0}, DTYPE), ({11: 256}, SHAPE), ({12: 32}, SHAPE), ({13: 8}, SHAPE), ({13: 0}, SHAPE), ({10: 65536}, SHAPE),
-    ({8: -1}, INVALID), ({10: 0}, INVALID), ({16: 3}, INVALID), ({17: -1}, INVALID), ({5: None, 9: 5}, INVALID),
+    ({8: -1}, INVALID), ({19: 0.0}, INVALID), ({19: float("nan")}, INVALID), ({10: 0}, INVALID), ({16: 3}, INVALID), ({17: -1}, INVALID), ({5: None, 9: 5}, INVALID),
     ({0: None}, INVALID), ({2: None}, INVALID), ({3: None}, INVALID), ({4: None}, INVALID), ({6: None}, INVALID),
     ({7: None}, INVALID), ({28: 568}, INVALID),
     ({2: 8}, MISALIGNED), ({20: 8193}, MISALIGNED), ({27: 9220}, MISALIGNED), ({0: 8}, MISALIGNED),

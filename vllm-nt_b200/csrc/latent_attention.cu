@@ -275,6 +275,46 @@ __device__ __forceinline__ uint64_t ring_desc(uint32_t saddr) {
   return d;
 }
 
+// Writes this warp's 32 latent columns of every M tile: row c to dst + row_at[c] (none if
+// negative), scaled by row_f[c].  Neighbouring lanes swap halves of two rows, so that a lane
+// stores two adjacent columns of one row; 16 rows' loads, products and stores are in flight
+// together.
+template <typename T, typename O, int N>
+__device__ __forceinline__ void write_rows(O* dst, uint32_t o_tmem, int quad, const float* row_f,
+                                           const int64_t* row_at) {
+  const int lane = threadIdx.x & 31;
+  const int odd = lane & 1;
+#pragma unroll 1
+  for (int c0 = 0; c0 < N; c0 += 16) {
+    float k[8];    // of the rows this lane stores: c0 + 2 i + odd
+    int64_t at[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      k[i] = row_f[c0 + 2 * i + odd];
+      at[i] = row_at[c0 + 2 * i + odd];
+    }
+#pragma unroll
+    for (int j = 0; j < kMTiles; ++j) {
+      const int col = j * 128 + quad * 32 + (lane & ~1);
+      uint32_t v[16];
+      __syncwarp();
+      tmem_ld_16(o_tmem + j * N + c0, v);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const uint32_t mine = odd ? v[2 * i + 1] : v[2 * i];
+        const uint32_t other = __shfl_xor_sync(0xffffffffu, odd ? v[2 * i] : v[2 * i + 1], 1);
+        float lo = __uint_as_float(odd ? other : mine) * k[i];
+        float hi = __uint_as_float(odd ? mine : other) * k[i];
+        if (k[i] == 0.f) lo = hi = 0.f;  // an empty row's O^T was never written
+        if (at[i] >= 0) {
+          if constexpr (sizeof(O) == 4) *reinterpret_cast<float2*>(dst + at[i] + col) = make_float2(lo, hi);
+          else Pair<T>::store(dst + at[i] + col, lo, hi);
+        }
+      }
+    }
+  }
+}
+
 template <typename T, int N>
 __global__ void __launch_bounds__(kThreads, 1)
     latent_attention_kernel(const __grid_constant__ CUtensorMap ql_map, const __grid_constant__ CUtensorMap qr_map,
@@ -564,7 +604,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             __syncwarp();
             tmem_ld_16x64(tmem + lanes + s * kTile, v);
 #pragma unroll
-            for (int i = 0; i < 32; ++i) x[i] = __uint_as_float(v[i]) * p.scale_log2;
+            for (int i = 0; i < 32; ++i) x[i] = __uint_as_float(v[i]);
           }
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
@@ -581,7 +621,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             for (int i = 0; i < 8; ++i) mx = fmaxf(mx, fmaxf(x[4 * i + 2 * h], x[4 * i + 2 * h + 1]));
             mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
             mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-            const float m_new = fmaxf(m[h], mx);
+            const float m_new = fmaxf(m[h], mx * p.scale_log2);  // the scale is positive
             if (m_new > m[h] + kRescaleLog2) {  // also true for the first finite maximum
               alpha[h] = hw_exp2(m[h] - m_new);
               m[h] = m_new;
@@ -607,8 +647,8 @@ __global__ void __launch_bounds__(kThreads, 1)
             float sum = 0.f;
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-              const float p0 = hw_exp2(x[4 * i + 2 * h] - m_use);
-              const float p1 = hw_exp2(x[4 * i + 2 * h + 1] - m_use);
+              const float p0 = hw_exp2(fmaf(x[4 * i + 2 * h], p.scale_log2, -m_use));
+              const float p1 = hw_exp2(fmaf(x[4 * i + 2 * h + 1], p.scale_log2, -m_use));
               sum += p0 + p1;
               Pair<T>::store(reinterpret_cast<T*>(&pk[2 * i + h]), p0, p1);
             }
@@ -691,25 +731,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       if (softmax_any(bad)) break;
       tc_fence_after();
-#pragma unroll 1
-      for (int j = 0; j < kMTiles; ++j) {
-        const int col = j * 128 + quad * 32 + lane;
-#pragma unroll 1
-        for (int c0 = 0; c0 < N; c0 += 16) {
-          uint32_t v[16];
-          __syncwarp();
-          tmem_ld_16(o_tmem + j * N + c0, v);
-#pragma unroll
-          for (int c = 0; c < 16; ++c) {
-            const float k = row_f[c0 + c];
-            const int64_t at = row_at[c0 + c];
-            if (at < 0) continue;
-            const float o = k == 0.f ? 0.f : __uint_as_float(v[c]) * k;  // an empty row's O^T was never written
-            if (whole) static_cast<T*>(p.out)[at + col] = Elem<T>::from_f(o);
-            else p.part_o[at + col] = o;
-          }
-        }
-      }
+      if (whole) write_rows<T, T, N>(static_cast<T*>(p.out), o_tmem, quad, row_f, row_at);
+      else write_rows<T, float, N>(p.part_o, o_tmem, quad, row_f, row_at);
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(&bars[L::kOFree]);  // the next piece may overwrite O^T
@@ -879,6 +902,7 @@ extern "C" int ntb200_latent_attention(
   if (num_seqs < 0 || num_tokens < 0 || num_heads <= 0 || num_blocks < 0 || max_blocks_per_seq < 0 ||
       block_table_stride < max_blocks_per_seq || max_query_len < 0)
     return fail(NTB200_ERR_INVALID_ARGUMENT, "latent_attention: bad sizes");
+  if (!(scale > 0.f)) return fail(NTB200_ERR_INVALID_ARGUMENT, "latent_attention: scale must be positive");
   if (query_start_loc == nullptr && num_seqs > 0 && num_tokens % num_seqs != 0)
     return fail(NTB200_ERR_INVALID_ARGUMENT, "latent_attention: without query_start_loc every sequence has num_tokens / num_seqs queries");
   if (num_seqs == 0 || num_tokens == 0 || (query_start_loc != nullptr && max_query_len == 0)) return NTB200_OK;
