@@ -93,7 +93,7 @@ struct LatentParams {
   float scale_log2;
   float* part_o;    // [ctas][2][64][512]
   float* part_lse;  // [ctas][2][64], log2
-  int4* desc;       // [ctas][2][2]
+  int4* desc;       // [ctas][2]: tiles before the share that ends an item (0: none), tiles a CTA; its rows
   unsigned int* err;
 };
 
@@ -142,24 +142,26 @@ struct Piece {
   __device__ __forceinline__ int valid(int t) const { return min(keys - t * kTile, kTile); }
 };
 
-// Walks a CTA's run of tiles; every role walks the same pieces.
+// Walks a CTA's run of tiles; every role walks the same pieces.  `s` is sequence b.
 struct Walk {
+  Seq s;
   int b, g, t;
   int64_t left;
   __device__ __forceinline__ bool next(const LatentParams& p, int team, Piece& o) {
-    while (left > 0 && b < p.num_seqs) {
-      o.s = sequence(p, b);
-      if (g >= o.s.groups) {
-        ++b;
+    while (left > 0) {
+      if (g >= s.groups) {
+        if (++b >= p.num_seqs) return false;
+        s = sequence(p, b);
         g = team;
         t = 0;
         continue;
       }
+      o.s = s;
       o.b = b;
       o.g = g;
       o.t0 = t;
-      o.keys = group_keys(p, o.s, g);
-      o.n = group_tiles(p, o.s, g);
+      o.keys = group_keys(p, s, g);
+      o.n = max((o.keys + kTile - 1) / kTile, 1);
       o.t1 = int64_t(o.n - t) < left ? o.n : t + int(left);
       left -= o.t1 - t;
       g += p.teams;
@@ -170,11 +172,31 @@ struct Walk {
   }
 };
 
-// tiles of sequence b that belong to this team
-__device__ __forceinline__ int64_t team_tiles(const LatentParams& p, int b, int team) {
-  const Seq s = sequence(p, b);
+// Tiles of sequence s that belong to this team.  With `skip` tiles to leave out: also the group
+// and the tile in it that come next (when there are that many).
+__device__ __forceinline__ int64_t team_tiles(const LatentParams& p, const Seq& s, int team, int64_t skip = -1,
+                                              int* at_group = nullptr, int* at_tile = nullptr) {
   int64_t n = 0;
-  for (int g = team; g < s.groups; g += p.teams) n += group_tiles(p, s, g);
+  if (p.teams > 1) {  // one group a sequence at most
+    if (team >= s.groups) return 0;
+    n = group_tiles(p, s, team);
+    if (skip >= 0 && skip < n) *at_group = team, *at_tile = int(skip);
+    return n;
+  }
+  int keys = s.ctx - s.q_len;
+  for (int g = 0, last = 0; g < s.groups; g += p.head_blocks) {
+    const int step = min(p.group_tokens, s.q_len - last);
+    last += step;
+    keys += step;
+    const int tiles = max((keys + kTile - 1) / kTile, 1);
+    const int64_t all = int64_t(tiles) * p.head_blocks;
+    if (skip >= n && skip < n + all) {
+      *at_group = g + int((skip - n) / tiles);
+      *at_tile = int((skip - n) % tiles);
+      return n;
+    }
+    n += all;
+  }
   return n;
 }
 
@@ -325,8 +347,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   float* const row_f = reinterpret_cast<float*>(smem + L::kRowF);
   int64_t* const row_at = reinterpret_cast<int64_t*>(smem + L::kRowAt);
   uint64_t* const bars = reinterpret_cast<uint64_t*>(smem + L::kBars);
-  int* const start = reinterpret_cast<int*>(smem + L::kStart);  // b, g, t of the run's first tile
-  uint32_t* const tmem_slot = reinterpret_cast<uint32_t*>(smem + L::kStart + 16);
+  int* const start = reinterpret_cast<int*>(smem + L::kStart);  // b, g, t of the run's first tile, its sequence
+  uint32_t* const tmem_slot = reinterpret_cast<uint32_t*>(smem + L::kStart + 28);
   int64_t* const scan = reinterpret_cast<int64_t*>(smem + L::kStart + 32);  // one a warp
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
@@ -336,15 +358,18 @@ __global__ void __launch_bounds__(kThreads, 1)
   pdl_wait();  // queries, cache and metadata come from the kernels before
 
   // ---- this CTA's run of its team's tiles ----
+  Seq own = {0, 0, 0, 0};  // this thread's first sequence
   int64_t mine = 0;
-  for (int b = threadIdx.x; b < p.num_seqs; b += kThreads) mine += team_tiles(p, b, team);
+  if (threadIdx.x < p.num_seqs) {
+    own = sequence(p, threadIdx.x);
+    mine = team_tiles(p, own, team);
+  }
+  const int64_t own_tiles = mine;
+  for (int b = threadIdx.x + kThreads; b < p.num_seqs; b += kThreads) mine += team_tiles(p, sequence(p, b), team);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
   if (lane == 0) scan[warp] = mine;
-  if (threadIdx.x < 2) {  // no share left behind yet
-    p.desc[(int64_t(blockIdx.x) * 2 + threadIdx.x) * 2] = make_int4(0, 0, 0, 0);
-    if (threadIdx.x == 0) start[0] = p.num_seqs;
-  }
+  if (threadIdx.x == 0) p.desc[int64_t(blockIdx.x) * 2] = make_int4(0, 0, 0, 0);  // ends no cut item yet
   __syncthreads();
   int64_t total = 0;
 #pragma unroll
@@ -357,7 +382,15 @@ __global__ void __launch_bounds__(kThreads, 1)
   int64_t carry = 0;
   for (int base = 0; base < p.num_seqs && carry <= begin; base += kThreads) {
     const int b = base + threadIdx.x;
-    const int64_t c = b < p.num_seqs ? team_tiles(p, b, team) : 0;
+    Seq sq = own;
+    int64_t c = own_tiles;
+    if (base > 0) {
+      c = 0;
+      if (b < p.num_seqs) {
+        sq = sequence(p, b);
+        c = team_tiles(p, sq, team);
+      }
+    }
     int64_t v = c;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -374,16 +407,10 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     const int64_t first = before + v - c;
     if (begin >= first && begin < first + c) {
-      const Seq s = sequence(p, b);
-      int64_t skip = begin - first;
-      int g = team;
-      while (skip >= group_tiles(p, s, g)) {
-        skip -= group_tiles(p, s, g);
-        g += p.teams;
-      }
-      start[0] = b;
-      start[1] = g;
-      start[2] = int(skip);
+      int g = 0, t = 0;
+      team_tiles(p, sq, team, begin - first, &g, &t);
+      start[0] = b, start[1] = g, start[2] = t;
+      start[3] = sq.q_begin, start[4] = sq.q_len, start[5] = sq.ctx, start[6] = sq.groups;
     }
     carry += sum;
     __syncthreads();
@@ -409,7 +436,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
-  Walk walk = {start[0], start[1], start[2], count};
+  Walk walk = {{start[3], start[4], start[5], start[6]}, start[0], start[1], start[2], count};
   Piece pc;
 
   if (warp == 0) {
@@ -425,6 +452,18 @@ __global__ void __launch_bounds__(kThreads, 1)
     uint32_t nq = 0, nu = 0;  // query loads and ring units so far
     bool ok = true;
     while (ok && walk.next(p, team, pc)) {
+      const int32_t* const bt = p.block_table + int64_t(pc.b) * p.bt_stride;
+      const int first = pc.t0 * kTileUnits;
+      const int last = (min(pc.keys, pc.t1 * kTile) + kUnit - 1) / kUnit;  // units [first, last) hold keys
+      // 32 units' page ids and groups at a time, one a lane, the next 32 fetched ahead
+      int page = -1, group = 0, next_page = -1, next_group = 0;
+      auto fetch = [&](int base) {
+        const int tok = (base + lane) * kUnit;
+        const int lb = tok / p.block_size;
+        next_group = (tok - lb * p.block_size) / 8;
+        next_page = base + lane < last ? __ldg(bt + lb) : 0;
+      };
+      fetch(first);
       const int qb = nq % L::kQBufs;
       uint64_t* const q_full = &bars[L::kQFull + qb];
       if (nq >= L::kQBufs && !mbar_wait_warp(&bars[L::kQEmpty + qb], (nq / L::kQBufs - 1) & 1, p.err)) break;
@@ -438,18 +477,6 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       __syncwarp();
       ++nq;
-      const int32_t* const bt = p.block_table + int64_t(pc.b) * p.bt_stride;
-      const int first = pc.t0 * kTileUnits;
-      const int last = (min(pc.keys, pc.t1 * kTile) + kUnit - 1) / kUnit;  // units [first, last) hold keys
-      // 32 units' page ids and groups at a time, one a lane, the next 32 fetched ahead
-      int page = -1, group = 0, next_page = -1, next_group = 0;
-      auto fetch = [&](int base) {
-        const int tok = (base + lane) * kUnit;
-        const int lb = tok / p.block_size;
-        next_group = (tok - lb * p.block_size) / 8;
-        next_page = base + lane < last ? __ldg(bt + lb) : 0;
-      };
-      fetch(first);
       // a tile is always four units of the ring, those past the last key empty
       const int end = (last + kTileUnits - 1) / kTileUnits * kTileUnits;
       for (int u = first; ok && u < end; ++u, ++nu) {
@@ -588,6 +615,9 @@ __global__ void __launch_bounds__(kThreads, 1)
         there[i] = active && rt < p.group_tokens && tok[i] < pc.s.q_len && head[i] < p.num_heads;
         limit[i] = there[i] ? max(pc.s.ctx - pc.s.q_len + tok[i] + 1, 0) : 0;  // sees keys [0, limit)
       }
+      // a cut item's share: the CTA's last piece begins it (t0 = 0), its first one continues it
+      const bool whole = pc.t0 == 0 && pc.t1 == pc.n;
+      const int64_t share = int64_t(blockIdx.x) * 2 + (pc.t0 == 0 ? 1 : 0);
       float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
       bool left = false;
       for (int t = pc.t0; t < pc.t1; ++t, ++g) {
@@ -634,6 +664,13 @@ __global__ void __launch_bounds__(kThreads, 1)
         __syncwarp();
         if (lane == 0) mbar_arrive(&bars[L::kSFree + s]);
         const bool news = softmax_any(grow || bad);
+        if (t == pc.t0 && active && (lane & 3) == 0) {  // (every warp has written the piece before out)
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+            row_at[r0 + 8 * h] = !there[h] ? -1
+                                 : whole   ? int64_t(pc.s.q_begin + tok[h]) * p.o_tok + int64_t(head[h]) * p.o_head
+                                           : (share * kMaxRows + r0 + 8 * h) * kLatent;
+        }
         if (news) {
           if ((lane & 3) == 0 && active) row_f[r0] = alpha[0], row_f[r0 + 8] = alpha[1];
           left = softmax_any(bad);
@@ -704,8 +741,6 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (left) break;
       // O^T is final once the piece's last product is complete
       bad = bad || !mbar_wait_warp(&bars[L::kPvDone], (g - 1) & 1, p.err);
-      const bool whole = pc.t0 == 0 && pc.t1 == pc.n;
-      const int64_t share = int64_t(blockIdx.x) * 2 + (pieces > 0 ? 1 : 0);
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const int row = r0 + 8 * h;
@@ -715,19 +750,14 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (active && (lane & 3) == 0) {
           const float lse2 = sum == 0.f ? -INFINITY : m[h] - kBias<T> + log2f(sum);
           row_f[row] = sum == 0.f ? 0.f : 1.f / sum;
-          if (whole) {
-            const int64_t at = int64_t(pc.s.q_begin + tok[h]);
-            row_at[row] = there[h] ? at * p.o_tok + int64_t(head[h]) * p.o_head : -1;
-            if (there[h] && p.lse != nullptr) p.lse[at * p.lse_tok + head[h]] = lse2 * 0.6931471805599453f;
-          } else {
-            row_at[row] = there[h] ? (share * kMaxRows + row) * kLatent : -1;
-            if (there[h]) p.part_lse[share * kMaxRows + row] = lse2;
-          }
+          if (!there[h]) continue;
+          if (!whole) p.part_lse[share * kMaxRows + row] = lse2;
+          else if (p.lse != nullptr) p.lse[int64_t(pc.s.q_begin + tok[h]) * p.lse_tok + head[h]] = lse2 * 0.6931471805599453f;
         }
       }
-      if (!whole && warp == kFirstSmWarp && lane == 0) {
-        p.desc[share * 2] = make_int4(1, pc.t0, pc.t1, pc.n);
-        p.desc[share * 2 + 1] = make_int4(pc.s.q_begin + tok0, pc.s.q_len - tok0, head0, int(min(per, int64_t(0x7fffffff))));
+      if (pc.t0 > 0 && pc.t1 == pc.n && warp == kFirstSmWarp && lane == 0) {  // this CTA ends a cut item
+        p.desc[int64_t(blockIdx.x) * 2] = make_int4(pc.t0, int(min(per, int64_t(0x7fffffff))), 0, 0);
+        p.desc[int64_t(blockIdx.x) * 2 + 1] = make_int4(pc.s.q_begin + tok0, pc.s.q_len - tok0, head0, 0);
       }
       if (softmax_any(bad)) break;
       tc_fence_after();
@@ -748,64 +778,62 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
 }
 
-// Joins the shares of every item that was cut.  The CTA whose first piece ends an item (its
-// share 0 has t0 > 0 and t1 = n) names that item.  Every CTA between the item's first and this one
-// had nothing else to do, so their number follows from t0 and the tiles a CTA.  A thread sums
-// four columns of a row over every fourth share; the four sums meet in shared memory.
-constexpr int kJoinCols = kLatent / 4;
-constexpr int kJoinParts = 4;
-constexpr int kJoinRows = 2;  // rows a CTA
+// Joins the shares of every item that was cut.  The CTA whose first piece ends an item names it;
+// every CTA between the item's first (whose last piece begins it) and this one had nothing else to
+// do, so their number follows from the tiles before and the tiles a CTA.  128 threads sum a row,
+// four columns each.
+constexpr int kJoinRows = 4;  // rows a block has at a time
+constexpr int kJoinLoops = 2;
+constexpr int kMaxCtas = 256;
 
 template <typename T>
-__global__ void __launch_bounds__(kJoinCols * kJoinParts) latent_join_kernel(const LatentParams p) {
-  __shared__ float4 sums[kJoinParts][kJoinCols];
-  __shared__ float weights[kJoinParts];
-  const int part = threadIdx.x / kJoinCols, col = threadIdx.x % kJoinCols;
+__global__ void __launch_bounds__(kJoinRows * 128) latent_join_kernel(const LatentParams p) {
+  __shared__ float weight[kJoinRows][kMaxCtas];
+  __shared__ float tops[kJoinRows][4];
+  const int slot = threadIdx.x >> 7, col = threadIdx.x & 127;
   pdl_trigger();
   pdl_wait();
   const int cta = blockIdx.x;
-  const int4 end = p.desc[int64_t(cta) * 4];
-  if (end.x == 0 || end.y == 0 || end.z != end.w) return;
-  const int4 where = p.desc[int64_t(cta) * 4 + 1];
-  const int n = 1 + (end.y + where.w - 1) / where.w;
+  const int4 end = p.desc[int64_t(cta) * 2];
+  const int4 where = p.desc[int64_t(cta) * 2 + 1];
+  if (end.x == 0) return;
+  const int n = 1 + (end.x + end.y - 1) / end.y;
   const int first = cta - (n - 1) * p.teams;
-  const int first_share = first * 2 + (p.desc[int64_t(first) * 4 + 2].x != 0 ? 1 : 0);
-  auto share = [&](int i) { return int64_t(i == 0 ? first_share : 2 * (first + i * p.teams)); };
-  for (int r = blockIdx.y * kJoinRows; r < (int(blockIdx.y) + 1) * kJoinRows; ++r) {
+  auto share = [&](int i) { return int64_t(i == 0 ? first * 2 + 1 : (first + i * p.teams) * 2); };
+#pragma unroll 1
+  for (int k = 0; k < kJoinLoops; ++k) {
+    const int r = (blockIdx.y * kJoinLoops + k) * kJoinRows + slot;
     const int tok = r / p.group_heads;
     const int head = where.z + r - tok * p.group_heads;
-    if (tok >= p.group_tokens || tok >= where.y || head >= p.num_heads) continue;
+    const bool there = tok < p.group_tokens && tok < where.y && head < p.num_heads;
     float top = -INFINITY;
-#pragma unroll 8
-    for (int i = 0; i < n; ++i) top = fmaxf(top, p.part_lse[share(i) * kMaxRows + r]);
-    const float ref = top == -INFINITY ? 0.f : top;
-    float sum = 0.f;
-    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 8
-    for (int i = part; i < n; i += kJoinParts) {
-      const int64_t row = share(i) * kMaxRows + r;
-      const float w = exp2f(p.part_lse[row] - ref);
-      const float4 o = reinterpret_cast<const float4*>(p.part_o + row * kLatent)[col];
-      sum += w;
-      acc.x += w * o.x, acc.y += w * o.y, acc.z += w * o.z, acc.w += w * o.w;
+    for (int i = col; there && i < n; i += 128) {
+      const float l = p.part_lse[share(i) * kMaxRows + r];
+      weight[slot][i] = l;
+      top = fmaxf(top, l);
     }
-    sums[part][col] = acc;
-    if (col == 0) weights[part] = sum;
-    __syncthreads();
-    if (part == 0) {
 #pragma unroll
-      for (int q = 1; q < kJoinParts; ++q) {
-        const float4 o = sums[q][col];
-        sum += weights[q];
-        acc.x += o.x, acc.y += o.y, acc.z += o.z, acc.w += o.w;
+    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    if ((col & 31) == 0) tops[slot][col >> 5] = top;
+    __syncthreads();
+    if (there) {
+      top = fmaxf(fmaxf(tops[slot][0], tops[slot][1]), fmaxf(tops[slot][2], tops[slot][3]));
+      const float ref = top == -INFINITY ? 0.f : top;
+      float sum = 0.f;
+      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 8
+      for (int i = 0; i < n; ++i) {
+        const float w = exp2f(weight[slot][i] - ref);
+        const float4 o = reinterpret_cast<const float4*>(p.part_o + (share(i) * kMaxRows + r) * kLatent)[col];
+        sum += w;
+        acc.x += w * o.x, acc.y += w * o.y, acc.z += w * o.z, acc.w += w * o.w;
       }
       const float inv = sum == 0.f ? 0.f : 1.f / sum;
       const float y[4] = {acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv};
       T* const o = static_cast<T*>(p.out) + int64_t(where.x + tok) * p.o_tok + int64_t(head) * p.o_head;
       *reinterpret_cast<Vec<T, 4>*>(o + col * 4) = pack_f<T, 4>(y);
       if (p.lse != nullptr && col == 0)
-        p.lse[int64_t(where.x + tok) * p.lse_tok + head] =
-            sum == 0.f ? -INFINITY : (ref + log2f(sum)) * 0.6931471805599453f;
+        p.lse[int64_t(where.x + tok) * p.lse_tok + head] = sum == 0.f ? -INFINITY : (ref + log2f(sum)) * 0.6931471805599453f;
     }
     __syncthreads();
   }
@@ -859,7 +887,7 @@ int launch_latent(const CUtensorMap& ql, const CUtensorMap& qr, const CUtensorMa
   if (st != NTB200_OK || p.team_ctas == 1) return st;  // one CTA a team cuts no item
   const int rows = p.group_heads * p.group_tokens;
   return launch_kernel("latent_attention (join)", latent_join_kernel<T>,
-                       dim3(ctas, unsigned(ceil_div(rows, kJoinRows))), dim3(kJoinCols * kJoinParts), 0, s, p);
+                       dim3(ctas, unsigned(ceil_div(rows, kJoinRows * kJoinLoops))), dim3(kJoinRows * 128), 0, s, p);
 }
 
 template <typename T>
@@ -874,7 +902,6 @@ int by_rows(const CUtensorMap& ql, const CUtensorMap& qr, const CUtensorMap& c, 
 constexpr int64_t kShareFloats = int64_t(kMaxRows) * kLatent;
 // per CTA: two shares of 64 x 512, their 64 log-sums, and their descriptors
 constexpr int64_t kBytesPerCta = 2 * (kShareFloats * 4 + kMaxRows * 4 + 32);
-constexpr int kMaxCtas = 1024;
 
 }  // namespace
 }  // namespace ntb200
