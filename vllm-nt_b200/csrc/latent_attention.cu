@@ -54,6 +54,7 @@ constexpr int kFirstSmWarp = 4;
 constexpr int kSmThreads = 128;
 constexpr int kThreads = 32 * kFirstSmWarp + kSmThreads;
 constexpr int kMaxTeams = 8;
+constexpr int kMaxCtas = 256;                    // one an SM
 constexpr float kRescaleLog2 = 8.0f;
 
 template <int N>
@@ -90,6 +91,7 @@ struct LatentParams {
   int block_size, num_blocks, max_blocks;
   int group_heads, head_blocks, group_tokens;  // rows of a group = group_heads * group_tokens
   int teams, team_ctas;
+  int64_t max_items;
   float scale_log2;
   float* part_o;    // [ctas][2][64][512]
   float* part_lse;  // [ctas][2][64], log2
@@ -191,8 +193,10 @@ __device__ __forceinline__ int64_t team_tiles(const LatentParams& p, const Seq& 
     const int tiles = max((keys + kTile - 1) / kTile, 1);
     const int64_t all = int64_t(tiles) * p.head_blocks;
     if (skip >= n && skip < n + all) {
-      *at_group = g + int((skip - n) / tiles);
-      *at_tile = int((skip - n) % tiles);
+      *at_group = g;
+      int64_t rest = skip - n;
+      for (; rest >= tiles; rest -= tiles) ++*at_group;
+      *at_tile = int(rest);
       return n;
     }
     n += all;
@@ -374,7 +378,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   int64_t total = 0;
 #pragma unroll
   for (int w = 0; w < kThreads / 32; ++w) total += scan[w];
-  const int64_t per = (total + p.team_ctas - 1) / p.team_ctas;
+  const int64_t per = total <= 0x7fffffff - kMaxCtas ? int64_t((int(total) + p.team_ctas - 1) / p.team_ctas)
+                                                     : (total + p.team_ctas - 1) / p.team_ctas;  // (slower)
   const int64_t begin = per * member;
   if (begin >= total) return;
   const int64_t count = min(per, total - begin);
@@ -778,56 +783,88 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
 }
 
-// Joins the shares of every item that was cut.  The CTA whose first piece ends an item names it;
-// every CTA between the item's first (whose last piece begins it) and this one had nothing else to
-// do, so their number follows from the tiles before and the tiles a CTA.  128 threads sum a row,
-// four columns each.
-constexpr int kJoinRows = 4;  // rows a block has at a time
-constexpr int kJoinLoops = 2;
-constexpr int kMaxCtas = 256;
+// Joins the shares of every item that was cut; block x takes the x-th CTA whose first piece ends
+// one.  Every CTA between the item's first (whose last piece begins it) and that one had nothing
+// else to do, so their number follows from the tiles before and the tiles a CTA.  128 threads sum
+// four columns each of a row.  PARTS = 4: a block's four sets of 128 share one row, each with every
+// fourth share (few items, so many shares each: 32 shares of 16 rows took 10 us on two SMs);
+// PARTS = 1: they take four rows, twice (many items, a few shares each).
+constexpr int kJoinSets = 4;
+constexpr int join_rows(int parts) { return parts == 1 ? 2 * kJoinSets : 1; }
 
-template <typename T>
-__global__ void __launch_bounds__(kJoinRows * 128) latent_join_kernel(const LatentParams p) {
-  __shared__ float weight[kJoinRows][kMaxCtas];
-  __shared__ float tops[kJoinRows][4];
-  const int slot = threadIdx.x >> 7, col = threadIdx.x & 127;
+template <typename T, int PARTS>
+__global__ void __launch_bounds__(kJoinSets * 128) latent_join_kernel(const LatentParams p) {
+  __shared__ float weight[kJoinSets][kMaxCtas];
+  __shared__ float tops[kJoinSets][4];
+  __shared__ float4 sums[PARTS == 1 ? 1 : kJoinSets][128];
+  __shared__ int ends[kJoinSets * 4], found;
+  const int set = threadIdx.x >> 7, col = threadIdx.x & 127;
   pdl_trigger();
   pdl_wait();
-  const int cta = blockIdx.x;
-  const int4 end = p.desc[int64_t(cta) * 2];
-  const int4 where = p.desc[int64_t(cta) * 2 + 1];
-  if (end.x == 0) return;
+  // ---- the x-th CTA that ends a cut item ----
+  const int ctas = p.teams * p.team_ctas;
+  const bool mine = threadIdx.x < ctas && p.desc[2 * threadIdx.x].x != 0;
+  const unsigned votes = __ballot_sync(0xffffffffu, mine);
+  if ((threadIdx.x & 31) == 0) ends[threadIdx.x >> 5] = __popc(votes);
+  if (threadIdx.x == 0) found = -1;
+  __syncthreads();
+  int before = __popc(votes & ((1u << (threadIdx.x & 31)) - 1));
+  for (int w = 0; w < (threadIdx.x >> 5); ++w) before += ends[w];
+  if (mine && before == blockIdx.x) found = threadIdx.x;
+  __syncthreads();
+  const int cta = found;
+  if (cta < 0) return;
+  const int4 end = p.desc[2 * cta];
+  const int4 where = p.desc[2 * cta + 1];
   const int n = 1 + (end.x + end.y - 1) / end.y;
   const int first = cta - (n - 1) * p.teams;
   auto share = [&](int i) { return int64_t(i == 0 ? first * 2 + 1 : (first + i * p.teams) * 2); };
 #pragma unroll 1
-  for (int k = 0; k < kJoinLoops; ++k) {
-    const int r = (blockIdx.y * kJoinLoops + k) * kJoinRows + slot;
+  for (int k = 0; k < (PARTS == 1 ? 2 : 1); ++k) {
+    const int r = blockIdx.y * join_rows(PARTS) + (PARTS == 1 ? k * kJoinSets + set : 0);
     const int tok = r / p.group_heads;
     const int head = where.z + r - tok * p.group_heads;
     const bool there = tok < p.group_tokens && tok < where.y && head < p.num_heads;
     float top = -INFINITY;
     for (int i = col; there && i < n; i += 128) {
       const float l = p.part_lse[share(i) * kMaxRows + r];
-      weight[slot][i] = l;
+      weight[set][i] = l;
       top = fmaxf(top, l);
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-    if ((col & 31) == 0) tops[slot][col >> 5] = top;
+    if ((col & 31) == 0) tops[set][col >> 5] = top;
+    __syncthreads();
+    top = fmaxf(fmaxf(tops[set][0], tops[set][1]), fmaxf(tops[set][2], tops[set][3]));
+    const float ref = top == -INFINITY ? 0.f : top;
+    float sum = 0.f;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (there) {
+      for (int i = col; i < n; i += 128) weight[set][i] = exp2f(weight[set][i] - ref);
+    }
     __syncthreads();
     if (there) {
-      top = fmaxf(fmaxf(tops[slot][0], tops[slot][1]), fmaxf(tops[slot][2], tops[slot][3]));
-      const float ref = top == -INFINITY ? 0.f : top;
-      float sum = 0.f;
-      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 8
-      for (int i = 0; i < n; ++i) {
-        const float w = exp2f(weight[slot][i] - ref);
+      for (int i = PARTS == 1 ? 0 : set; i < n; i += PARTS) {
+        const float w = weight[set][i];
         const float4 o = reinterpret_cast<const float4*>(p.part_o + (share(i) * kMaxRows + r) * kLatent)[col];
         sum += w;
         acc.x += w * o.x, acc.y += w * o.y, acc.z += w * o.z, acc.w += w * o.w;
       }
+    }
+    if constexpr (PARTS > 1) {
+      sums[set][col] = acc;
+      if (col == 0) tops[set][0] = sum;
+      __syncthreads();
+      if (set > 0) return;
+#pragma unroll
+      for (int q = 1; q < PARTS; ++q) {
+        const float4 o = sums[q][col];
+        sum += tops[q][0];
+        acc.x += o.x, acc.y += o.y, acc.z += o.z, acc.w += o.w;
+      }
+    }
+    if (there) {
       const float inv = sum == 0.f ? 0.f : 1.f / sum;
       const float y[4] = {acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv};
       T* const o = static_cast<T*>(p.out) + int64_t(where.x + tok) * p.o_tok + int64_t(head) * p.o_head;
@@ -835,7 +872,7 @@ __global__ void __launch_bounds__(kJoinRows * 128) latent_join_kernel(const Late
       if (p.lse != nullptr && col == 0)
         p.lse[int64_t(where.x + tok) * p.lse_tok + head] = sum == 0.f ? -INFINITY : (ref + log2f(sum)) * 0.6931471805599453f;
     }
-    __syncthreads();
+    if constexpr (PARTS == 1) __syncthreads();
   }
 }
 
@@ -885,9 +922,13 @@ int launch_latent(const CUtensorMap& ql, const CUtensorMap& qr, const CUtensorMa
   st = launch_kernel("latent_attention", latent_attention_kernel<T, N>, dim3(ctas), dim3(kThreads), Layout<N>::kBytes,
                      s, ql, qr, c, p);
   if (st != NTB200_OK || p.team_ctas == 1) return st;  // one CTA a team cuts no item
-  const int rows = p.group_heads * p.group_tokens;
-  return launch_kernel("latent_attention (join)", latent_join_kernel<T>,
-                       dim3(ctas, unsigned(ceil_div(rows, kJoinRows * kJoinLoops))), dim3(kJoinRows * 128), 0, s, p);
+  // blocks for as many items as can be cut; one row each where an item has over three shares on average
+  const unsigned rows = unsigned(p.group_heads * p.group_tokens);
+  const unsigned items = unsigned(std::min<int64_t>(p.max_items, ctas));
+  if (ctas > 3 * items)
+    return launch_kernel("latent_attention (join)", latent_join_kernel<T, 4>, dim3(items, rows), dim3(kJoinSets * 128), 0, s, p);
+  return launch_kernel("latent_attention (join)", latent_join_kernel<T, 1>,
+                       dim3(items, unsigned(ceil_div(rows, join_rows(1)))), dim3(kJoinSets * 128), 0, s, p);
 }
 
 template <typename T>
@@ -975,6 +1016,7 @@ extern "C" int ntb200_latent_attention(
   p.err = device_error_word();
   const int64_t groups = ceil_div(p.max_query, p.group_tokens) * p.head_blocks;
   p.teams = groups <= kMaxTeams ? int(groups) : 1;
+  p.max_items = groups * num_seqs;
   const int64_t cap = max_blocks_per_seq * block_size;
   const int64_t keys = max_seq_len > 0 && max_seq_len < cap ? max_seq_len : cap;
   // no more CTAs than the batch can have tiles
