@@ -226,33 +226,6 @@ constexpr float kBias = 0.f;
 template <>
 constexpr float kBias<__half> = 7.f;
 
-// The lane that issues for a converged warp, and instructions that only it issues.
-__device__ __forceinline__ uint32_t elect_one() {
-  uint32_t e;
-  asm volatile(
-      "{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}"
-      : "=r"(e));
-  return e;
-}
-__device__ __forceinline__ void umma_elected(uint32_t tmem_d, uint64_t a, uint64_t b, uint32_t idesc,
-                                             uint32_t accumulate, uint32_t elected) {
-  asm volatile(
-      "{\n\t.reg .pred p, q;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "setp.ne.b32 q, %5, 0;\n\t"
-      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(tmem_d),
-      "l"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(elected)
-      : "memory");
-}
-__device__ __forceinline__ void commit_elected(uint64_t* bar, uint32_t elected) {
-  asm volatile(
-      "{\n\t.reg .pred q;\n\t"
-      "setp.ne.b32 q, %1, 0;\n\t"
-      "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(smem_u32(bar)),
-      "r"(elected)
-      : "memory");
-}
-
 __device__ __forceinline__ void tma_load_5d(uint32_t dst, const CUtensorMap* map, int group, int block, uint32_t bar) {
   asm volatile(
       "cp.async.bulk.tensor.5d.shared::cluster.global.tile.mbarrier::complete_tx::bytes "

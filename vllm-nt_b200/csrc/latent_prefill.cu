@@ -139,16 +139,6 @@ struct Walk {
   }
 };
 
-__device__ __forceinline__ void umma_f16_tmem_a(uint32_t tmem_d, uint32_t tmem_a, uint64_t bdesc, uint32_t idesc,
-                                                uint32_t accumulate) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(tmem_d),
-      "r"(tmem_a), "l"(bdesc), "r"(idesc), "r"(accumulate)
-      : "memory");
-}
-
 __device__ __forceinline__ void tmem_st_16(uint32_t taddr, const uint32_t (&r)[16]) {
   asm volatile(
       "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
@@ -213,159 +203,157 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   if (warp == kTmaWarp) {
     // ------------------------------ TMA producer ------------------------------
+    const uint32_t elected = elect_one();
+    if (elected) {
+      asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&q_map)) : "memory");
+      asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&kn_map)) : "memory");
+      asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&kr_map)) : "memory");
+      asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&v_map)) : "memory");
+    }
+    __syncwarp();
     uint32_t nq[2] = {0, 0};  // Q tiles loaded
     uint32_t n = 0;           // ring chunks loaded
     bool ok = true;
     for (int64_t w = blockIdx.x; ok && walk.get(p, w, it); w += gridDim.x) {
-      if (lane == 0) {
-        auto load_q = [&](int x) {
-          if (it.tiles[x] == 0) return;
-          uint64_t* const full = &bars[Smem::kQFull + x];
-          if (nq[x] >= 1 && !mbar_wait(&bars[Smem::kQEmpty + x], (nq[x] - 1) & 1, p.err)) {
-            ok = false;
-            return;
-          }
+      auto load_q = [&](int x) {
+        if (!ok || it.tiles[x] == 0) return;
+        uint64_t* const full = &bars[Smem::kQFull + x];
+        if (nq[x] >= 1) ok = mbar_wait_warp(&bars[Smem::kQEmpty + x], (nq[x] - 1) & 1, p.err);
+        if (!ok) return;
+        if (elected) {
           mbar_arrive_expect_tx(full, kQChunks * kChunkBytes);
           for (int c = 0; c < kQChunks; ++c)
             tma_load_3d(sm + Smem::kQ + (x * kQChunks + c) * kChunkBytes, &q_map, c * 64, it.head,
                         it.q_begin + it.q0 + x * kBQ, smem_u32(full));
-          ++nq[x];
-        };
-        auto slot = [&]() -> uint64_t* {
+        }
+        __syncwarp();
+        ++nq[x];
+      };
+      const int tiles = max(it.tiles[0], it.tiles[1]);
+      load_q(0);
+      for (int j = 0; ok && j < tiles; ++j) {
+        const int row = it.k_begin + j * kBK;
+#pragma unroll 1
+        for (int c = 0; ok && c < kQChunks + kVChunks; ++c) {
           const uint32_t s = n % kRing;
-          if (n >= kRing && !mbar_wait(&bars[Smem::kEmpty + s], (n / kRing - 1) & 1, p.err)) {
-            ok = false;
-            return nullptr;
-          }
-          mbar_arrive_expect_tx(&bars[Smem::kFull + s], kChunkBytes);
-          return &bars[Smem::kFull + s];
-        };
-        const int tiles = max(it.tiles[0], it.tiles[1]);
-        load_q(0);
-        for (int j = 0; ok && j < tiles; ++j) {
-          const int row = it.k_begin + j * kBK;
-          for (int c = 0; ok && c < kQChunks; ++c) {
-            uint64_t* const full = slot();
-            if (full == nullptr) break;
-            const uint32_t dst = sm + Smem::kKv + (n % kRing) * kChunkBytes;
+          if (n >= kRing) ok = mbar_wait_warp(&bars[Smem::kEmpty + s], (n / kRing - 1) & 1, p.err);
+          if (!ok) break;
+          if (elected) {
+            uint64_t* const full = &bars[Smem::kFull + s];
+            const uint32_t dst = sm + Smem::kKv + s * kChunkBytes;
+            mbar_arrive_expect_tx(full, kChunkBytes);
             if (c < kNope / 64) tma_load_3d(dst, &kn_map, c * 64, it.head, row, smem_u32(full));
-            else tma_load_2d(dst, &kr_map, 0, row, smem_u32(full));
-            ++n;
+            else if (c < kQChunks) tma_load_2d(dst, &kr_map, 0, row, smem_u32(full));
+            else tma_load_3d(dst, &v_map, (c - kQChunks) * 64, it.head, row, smem_u32(full));
           }
-          if (ok && j == 0) load_q(1);
-          for (int c = 0; ok && c < kVChunks; ++c) {
-            uint64_t* const full = slot();
-            if (full == nullptr) break;
-            tma_load_3d(sm + Smem::kKv + (n % kRing) * kChunkBytes, &v_map, c * 64, it.head, row, smem_u32(full));
-            ++n;
-          }
+          __syncwarp();
+          ++n;
+          if (j == 0 && c == kQChunks - 1) load_q(1);
         }
       }
-      ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
     }
-    if (lane == 0) {
-      // drain the copies that may still be in flight
-      for (int x = 0; x < 2; ++x)
-        if (nq[x] > 0) mbar_wait(&bars[Smem::kQFull + x], (nq[x] - 1) & 1, p.err);
-      for (uint32_t i = n > kRing ? n - kRing : 0; i < n; ++i)
-        mbar_wait(&bars[Smem::kFull + i % kRing], (i / kRing) & 1, p.err);
-    }
+    // drain the copies that may still be in flight
+    for (int x = 0; x < 2; ++x)
+      if (nq[x] > 0) mbar_wait_warp(&bars[Smem::kQFull + x], (nq[x] - 1) & 1, p.err);
+    for (uint32_t i = n > kRing ? n - kRing : 0; i < n; ++i)
+      mbar_wait_warp(&bars[Smem::kFull + i % kRing], (i / kRing) & 1, p.err);
   } else if (warp == kSWarp) {
     // -------------------------- MMA issuer: S = Q K^T --------------------------
+    const uint32_t elected = elect_one();
     const uint32_t idesc = make_idesc(std::is_same<T, __nv_bfloat16>::value, kBQ, kBK);
     uint32_t ns[2] = {0, 0};  // products issued a tile
     uint32_t nq[2] = {0, 0};
     uint32_t n = 0;  // ring chunks passed (V's among them)
     bool ok = true;
     for (int64_t w = blockIdx.x; ok && walk.get(p, w, it); w += gridDim.x) {
-      if (lane == 0) {
-        const int tiles = max(it.tiles[0], it.tiles[1]);
-        for (int j = 0; ok && j < tiles; ++j, n += kQChunks + kVChunks) {
+      const int tiles = max(it.tiles[0], it.tiles[1]);
+      for (int j = 0; ok && j < tiles; ++j, n += kQChunks + kVChunks) {
 #pragma unroll
-          for (int x = 0; x < 2; ++x) {
-            if (!ok || j >= it.tiles[x]) continue;
-            const bool last_user = x == 1 || j >= it.tiles[1];
-            // the buffer's weights of the tile before have been used up
-            if ((j == 0 && !mbar_wait(&bars[Smem::kQFull + x], nq[x] & 1, p.err)) ||
-                (ns[x] >= 1 && !mbar_wait(&bars[Smem::kPvDone + x], (ns[x] - 1) & 1, p.err))) {
-              ok = false;
-              continue;
-            }
-            for (int c = 0; c < kQChunks; ++c) {
-              const uint32_t s = (n + c) % kRing;
-              if (!mbar_wait(&bars[Smem::kFull + s], ((n + c) / kRing) & 1, p.err)) {
-                ok = false;
-                break;
-              }
-              tc_fence_after();
-              const uint64_t a = sw128_kmajor_desc(sm + Smem::kQ + (x * kQChunks + c) * kChunkBytes);
-              const uint64_t b = sw128_kmajor_desc(sm + Smem::kKv + s * kChunkBytes);
+        for (int x = 0; x < 2; ++x) {
+          if (!ok || j >= it.tiles[x]) continue;
+          const bool last_user = x == 1 || j >= it.tiles[1];
+          // the buffer's weights of the tile before have been used up
+          ok = (j > 0 || mbar_wait_warp(&bars[Smem::kQFull + x], nq[x] & 1, p.err)) &&
+               (ns[x] == 0 || mbar_wait_warp(&bars[Smem::kPvDone + x], (ns[x] - 1) & 1, p.err));
+          const uint64_t a0 = sw128_kmajor_desc(sm + Smem::kQ + x * kQChunks * kChunkBytes);
+          const uint64_t b0 = sw128_kmajor_desc(sm + Smem::kKv);
 #pragma unroll
-              for (int k = 0; k < 4; ++k) umma_f16(tmem + x * kBK, a + 2 * k, b + 2 * k, idesc, (c | k) ? 1u : 0u);
-              if (last_user) umma_commit(&bars[Smem::kEmpty + s]);
-            }
-            umma_commit(&bars[Smem::kSFull + x]);
-            ++ns[x];
-            if (j + 1 == it.tiles[x]) {
-              umma_commit(&bars[Smem::kQEmpty + x]);
-              ++nq[x];
-            }
+          for (int c = 0; c < kQChunks; ++c) {
+            const uint32_t s = (n + c) % kRing;
+            ok = ok && mbar_wait_warp(&bars[Smem::kFull + s], ((n + c) / kRing) & 1, p.err);
+            if (!ok) break;
+            tc_fence_after();
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              umma_elected(tmem + x * kBK, a0 + c * (kChunkBytes >> 4) + 2 * k, b0 + s * (kChunkBytes >> 4) + 2 * k, idesc,
+                           (c | k) ? 1u : 0u, elected);
+            if (last_user) commit_elected(&bars[Smem::kEmpty + s], elected);
+          }
+          if (!ok) continue;
+          commit_elected(&bars[Smem::kSFull + x], elected);
+          ++ns[x];
+          if (j + 1 == it.tiles[x]) {
+            commit_elected(&bars[Smem::kQEmpty + x], elected);
+            ++nq[x];
           }
         }
       }
-      ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
     }
-    if (lane == 0) {
-      // every issued MMA completes before TMEM may be released
-      umma_commit(&bars[Smem::kMmaDone]);
-      mbar_wait(&bars[Smem::kMmaDone], 0, p.err);
-    }
+    // every issued MMA completes before TMEM may be released
+    commit_elected(&bars[Smem::kMmaDone], elected);
+    mbar_wait_warp(&bars[Smem::kMmaDone], 0, p.err);
   } else if (warp == kPvWarp) {
     // -------------------------- MMA issuer: O += P V --------------------------
-    const uint32_t idesc = make_idesc(std::is_same<T, __nv_bfloat16>::value, kBQ, 64) | (1u << 16);  // B (V) MN-major
+    const uint32_t elected = elect_one();
+    constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
+    const uint32_t idesc = make_idesc(kBf16, kBQ, kV) | (1u << 16);       // B (V) MN-major
+    const uint32_t idesc_half = make_idesc(kBf16, kBQ, 64) | (1u << 16);  // one chunk of it
     uint32_t np[2] = {0, 0};     // products issued a tile
     uint32_t items[2] = {0, 0};  // outputs begun
     uint32_t n = 0;
     bool ok = true;
     for (int64_t w = blockIdx.x; ok && walk.get(p, w, it); w += gridDim.x) {
-      if (lane == 0) {
-        const int tiles = max(it.tiles[0], it.tiles[1]);
-        for (int j = 0; ok && j < tiles; ++j, n += kQChunks + kVChunks) {
-          const int steps = (min(it.ctx - j * kBK, kBK) + 15) / 16;
+      const int tiles = max(it.tiles[0], it.tiles[1]);
+      for (int j = 0; ok && j < tiles; ++j, n += kQChunks + kVChunks) {
+        const int steps = (min(it.ctx - j * kBK, kBK) + 15) / 16;
+        const uint32_t s0 = (n + kQChunks) % kRing, s1 = (n + kQChunks + 1) % kRing;
+        const uint64_t v0 = sw128_mnmajor_desc(sm + Smem::kKv + s0 * kChunkBytes, kChunkBytes);
+        const uint64_t v1 = sw128_mnmajor_desc(sm + Smem::kKv + s1 * kChunkBytes, kChunkBytes);
 #pragma unroll
-          for (int x = 0; x < 2; ++x) {
-            if (!ok || j >= it.tiles[x]) continue;
-            const bool last_user = x == 1 || j >= it.tiles[1];
-            if (!mbar_wait(&bars[Smem::kPFull + x], np[x] & 1, p.err) ||
-                (j == 0 && items[x] >= 1 && !mbar_wait(&bars[Smem::kOFree + x], (items[x] - 1) & 1, p.err))) {
-              ok = false;
-              continue;
-            }
-            for (int c = 0; c < kVChunks; ++c) {
-              const uint32_t at = n + kQChunks + c, s = at % kRing;
-              if (!mbar_wait(&bars[Smem::kFull + s], (at / kRing) & 1, p.err)) {
-                ok = false;
-                break;
+        for (int x = 0; x < 2; ++x) {
+          if (!ok || j >= it.tiles[x]) continue;
+          const bool last_user = x == 1 || j >= it.tiles[1];
+          ok = mbar_wait_warp(&bars[Smem::kPFull + x], np[x] & 1, p.err) &&
+               (j > 0 || items[x] == 0 || mbar_wait_warp(&bars[Smem::kOFree + x], (items[x] - 1) & 1, p.err)) &&
+               mbar_wait_warp(&bars[Smem::kFull + s0], ((n + kQChunks) / kRing) & 1, p.err) &&
+               mbar_wait_warp(&bars[Smem::kFull + s1], ((n + kQChunks + 1) / kRing) & 1, p.err);
+          if (!ok) continue;
+          tc_fence_after();
+          const uint32_t o_tmem = tmem + kTmemO + x * kV, p_tmem = tmem + x * kBK;
+          if (s1 == s0 + 1) {  // both chunks of V lie together: one product over 128 columns
+#pragma unroll
+            for (int k = 0; k < kBK / 16; ++k)
+              if (k < steps) umma_tmem_a_elected(o_tmem, p_tmem + k * 8, v0 + k * (2048 >> 4), idesc, (j > 0 || k > 0) ? 1u : 0u, elected);
+          } else {             // the ring wraps between them
+#pragma unroll
+            for (int k = 0; k < kBK / 16; ++k)
+              if (k < steps) {
+                umma_tmem_a_elected(o_tmem, p_tmem + k * 8, v0 + k * (2048 >> 4), idesc_half, (j > 0 || k > 0) ? 1u : 0u, elected);
+                umma_tmem_a_elected(o_tmem + 64, p_tmem + k * 8, v1 + k * (2048 >> 4), idesc_half, (j > 0 || k > 0) ? 1u : 0u, elected);
               }
-              tc_fence_after();
-              const uint32_t vb = sm + Smem::kKv + s * kChunkBytes;
-              for (int k = 0; k < steps; ++k)
-                umma_f16_tmem_a(tmem + kTmemO + x * kV + c * 64, tmem + x * kBK + k * 8,
-                                sw128_mnmajor_desc(vb + k * 2048, kChunkBytes), idesc, (j > 0 || k > 0) ? 1u : 0u);
-              if (last_user) umma_commit(&bars[Smem::kEmpty + s]);
-            }
-            umma_commit(&bars[Smem::kPvDone + x]);
-            ++np[x];
-            if (j == 0) ++items[x];
           }
+          if (last_user) {
+            commit_elected(&bars[Smem::kEmpty + s0], elected);
+            commit_elected(&bars[Smem::kEmpty + s1], elected);
+          }
+          commit_elected(&bars[Smem::kPvDone + x], elected);
+          ++np[x];
+          if (j == 0) ++items[x];
         }
       }
-      ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
     }
-    if (lane == 0) {
-      umma_commit(&bars[Smem::kMmaDone]);
-      mbar_wait(&bars[Smem::kMmaDone], 0, p.err);
-    }
+    commit_elected(&bars[Smem::kMmaDone], elected);
+    mbar_wait_warp(&bars[Smem::kMmaDone], 0, p.err);
   } else if (warp < 8) {
     // ------------------------------ softmax + output ------------------------------
     const int x = warp >> 2;
