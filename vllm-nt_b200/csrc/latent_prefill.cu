@@ -36,6 +36,11 @@ constexpr int kRing = 8;
 constexpr int kThreads = 384;
 constexpr int kSWarp = 8, kPvWarp = 9, kTmaWarp = 10, kAllocWarp = 11;
 constexpr float kRescaleLog2 = 8.0f;
+// of every kEmulateOf pairs of weights kEmulated are taken on the FMA pipe
+constexpr int kEmulateOf = 4, kEmulated = 1;
+// registers: launched with 168 a thread, the two softmax warpgroups draw what the third gives up
+constexpr int kSoftmaxRegs = 208, kIssueRegs = 88;
+static_assert(256 * kSoftmaxRegs + 128 * kIssueRegs <= 384 * 168, "register split");
 constexpr uint32_t kTmemCols = 512;
 constexpr uint32_t kTmemO = 256;  // S_A, S_B at 0, 128; O_A, O_B at 256, 384
 
@@ -154,6 +159,81 @@ __device__ __forceinline__ float hw_exp2(float x) {
   return y;
 }
 
+// 32 TMEM columns on their way into registers, which are there once tmem_ld_done has named them.
+__device__ __forceinline__ void tmem_ld_32_begin(uint32_t taddr, uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_ld_done(uint32_t (&r)[32]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+                 "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]),
+                 "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]),
+                 "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]),
+                 "+r"(r[30]), "+r"(r[31])::"memory");
+}
+
+// Two fp32 values in one register pair, and operations on both.
+__device__ __forceinline__ uint64_t pack2f(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void unpack2f(uint64_t v, float& a, float& b) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v));
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
+// 2^y of two values on the FMA pipe: y = n + f with n whole and |f| <= 1/2, 2^f by a polynomial of
+// degree 5 (least squares of the relative error with the largest errors reweighted, the constant
+// term 1: off by 1.7e-7 in fp32), times 2^n from n's bits.  The hardware's exponentials take 8 cycles
+// a warp, 2048 of the 2560 that the tensor core needs for a pair of tiles; these are for the share
+// of them that the FMA pipe has room for.  y <= 127; below -126.5, -inf included, the result is 0;
+// a NaN stays one.
+__device__ __forceinline__ void fma_exp2(uint64_t y, float& a, float& b) {
+  float y0, y1;
+  unpack2f(y, y0, y1);
+  y = pack2f(max_nan(y0, -127.f), max_nan(y1, -127.f));
+  const float big = 12582912.f + 127.f;  // 1.5 * 2^23: the sum's low bits are n + 127
+  const uint64_t t = add2(y, pack2f(big, big));
+  const uint64_t f = add2(y, mul2(add2(t, pack2f(-big, -big)), pack2f(-1.f, -1.f)));
+  uint64_t q = fma2(f, pack2f(0.001326472731307149f, 0.001326472731307149f), pack2f(0.009671512991189957f, 0.009671512991189957f));
+  q = fma2(q, f, pack2f(0.05550733581185341f, 0.05550733581185341f));
+  q = fma2(q, f, pack2f(0.24022242426872253f, 0.24022242426872253f));
+  q = fma2(q, f, pack2f(0.6931470036506653f, 0.6931470036506653f));
+  q = fma2(q, f, pack2f(1.f, 1.f));
+  float t0, t1;
+  unpack2f(t, t0, t1);
+  q = mul2(q, pack2f(__uint_as_float(__float_as_uint(t0) << 23), __uint_as_float(__float_as_uint(t1) << 23)));
+  unpack2f(q, a, b);
+}
+
 // The running maximum is subtracted less kBias: fp16 weights then span 2^7 .. 2^15 at the
 // row's largest score and reach 2^-31 of it before they vanish (bf16 has fp32's range).
 template <typename T>
@@ -201,6 +281,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   Item it;
   walk.begin(p);
 
+  if (warp >= 8) {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kIssueRegs));
   if (warp == kTmaWarp) {
     // ------------------------------ TMA producer ------------------------------
     const uint32_t elected = elect_one();
@@ -354,22 +436,24 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     commit_elected(&bars[Smem::kMmaDone], elected);
     mbar_wait_warp(&bars[Smem::kMmaDone], 0, p.err);
-  } else if (warp < 8) {
+  }
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
     // ------------------------------ softmax + output ------------------------------
-    const int x = warp >> 2;
+    const int x_tile = warp >> 2;
     const int r = (warp & 3) * 32 + lane;
     const uint32_t lanes = uint32_t((warp & 3) * 32) << 16;
-    const uint32_t s_tmem = tmem + x * kBK + lanes;
-    const uint32_t o_tmem = tmem + kTmemO + x * kV + lanes;
+    const uint32_t s_tmem = tmem + x_tile * kBK + lanes;
+    const uint32_t o_tmem = tmem + kTmemO + x_tile * kV + lanes;
     uint32_t g = 0;  // key tiles done
     uint32_t n = 0;  // ring chunks passed
     bool ok = true;
     for (int64_t w = blockIdx.x; ok && walk.get(p, w, it); w += gridDim.x) {
-      const int qi = it.q0 + x * kBQ + r;
-      const bool there = r < it.rows[x];
+      const int qi = it.q0 + x_tile * kBQ + r;
+      const bool there = r < it.rows[x_tile];
       const int64_t tok = it.q_begin + qi;
       T* const orow = static_cast<T*>(p.out) + tok * p.o_tok + int64_t(it.head) * p.o_head;
-      const int tiles = it.tiles[x];
+      const int tiles = it.tiles[x_tile];
       const int both = max(it.tiles[0], it.tiles[1]);
       if (tiles == 0) {  // no visible key: zero rows, as for an empty softmax
         if (there) {
@@ -384,27 +468,29 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int limit = !there ? 0 : p.causal ? min(max(it.ctx - it.q_len + qi + 1, 0), it.ctx) : it.ctx;
       float m = -INFINITY, l = 0.f;
       for (int j = 0; j < tiles; ++j, ++g) {
-        if (!mbar_wait_warp(&bars[Smem::kSFull + x], g & 1, p.err)) {
+        if (!mbar_wait_warp(&bars[Smem::kSFull + x_tile], g & 1, p.err)) {
           ok = false;
           break;
         }
         tc_fence_after();
         const int seen = limit - j * kBK;  // columns i < seen are visible
+        uint32_t x[kBK / 32][32];
+        __syncwarp();
+#pragma unroll
+        for (int c = 0; c < kBK / 32; ++c) tmem_ld_32_begin(s_tmem + c * 32, x[c]);
         // ---- the tile's maximum ----
         float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
         for (int c = 0; c < kBK / 32; ++c) {
-          uint32_t v[32];
-          __syncwarp();
-          tmem_ld_32(s_tmem + c * 32, v);
-          if (seen >= (c + 1) * 32) {
-#pragma unroll
-            for (int i = 0; i < 32; ++i) m4[i & 3] = fmaxf(m4[i & 3], __uint_as_float(v[i]));
-          } else {
+          tmem_ld_done(x[c]);
+          if (seen < (c + 1) * 32) {
 #pragma unroll
             for (int i = 0; i < 32; ++i)
-              m4[i & 3] = fmaxf(m4[i & 3], c * 32 + i < seen ? __uint_as_float(v[i]) : -INFINITY);
+              if (c * 32 + i >= seen) x[c][i] = 0xff800000u;  // -inf
           }
+#pragma unroll
+          for (int i = 0; i < 32; i += 2)
+            m4[(i >> 1) & 3] = fmaxf(fmaxf(m4[(i >> 1) & 3], __uint_as_float(x[c][i])), __uint_as_float(x[c][i + 1]));
         }
         // (the scale is positive, so the largest score is the largest scaled one)
         const float top = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * p.scale_log2;
@@ -415,7 +501,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (up) m = m_new;
           l *= alpha;
           if (j > 0) {
-            if (!mbar_wait_warp(&bars[Smem::kPvDone + x], (g - 1) & 1, p.err)) {
+            if (!mbar_wait_warp(&bars[Smem::kPvDone + x_tile], (g - 1) & 1, p.err)) {
               ok = false;
               break;
             }
@@ -433,29 +519,32 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         // ---- the weights, over the scores they come from ----
         const float m_use = m == -INFINITY ? 0.f : m - kBias<T>;
-        float l4[4] = {0.f, 0.f, 0.f, 0.f};
+        const uint64_t scale2 = pack2f(p.scale_log2, p.scale_log2), minus_m = pack2f(-m_use, -m_use);
+        uint64_t l2[2] = {0, 0};
 #pragma unroll
         for (int c = 0; c < kBK / 32; ++c) {
-          uint32_t v[32], pk[16];
-          __syncwarp();
-          tmem_ld_32(s_tmem + c * 32, v);
-          float e[32];
-          if (seen >= (c + 1) * 32) {
-#pragma unroll
-            for (int i = 0; i < 32; ++i) e[i] = hw_exp2(fmaf(__uint_as_float(v[i]), p.scale_log2, -m_use));
-          } else {
-#pragma unroll
-            for (int i = 0; i < 32; ++i)
-              e[i] = c * 32 + i < seen ? hw_exp2(fmaf(__uint_as_float(v[i]), p.scale_log2, -m_use)) : 0.f;
-          }
+          uint32_t pk[16];
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
-            l4[i & 3] += e[2 * i] + e[2 * i + 1];
-            Pair<T>::store(reinterpret_cast<T*>(&pk[i]), e[2 * i], e[2 * i + 1]);
+            const uint64_t y = fma2(pack2f(__uint_as_float(x[c][2 * i]), __uint_as_float(x[c][2 * i + 1])), scale2, minus_m);
+            float e0, e1;
+            if (i % kEmulateOf >= kEmulateOf - kEmulated) {
+              fma_exp2(y, e0, e1);
+            } else {
+              unpack2f(y, e0, e1);
+              e0 = hw_exp2(e0);
+              e1 = hw_exp2(e1);
+            }
+            l2[i & 1] = add2(l2[i & 1], pack2f(e0, e1));
+            Pair<T>::store(reinterpret_cast<T*>(&pk[i]), e0, e1);
           }
           tmem_st_16(s_tmem + c * 16, pk);
         }
-        l += (l4[0] + l4[1]) + (l4[2] + l4[3]);
+        {
+          float a, b;
+          unpack2f(add2(l2[0], l2[1]), a, b);
+          l += a + b;
+        }
         asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
         const int inside = it.ctx - j * kBK;  // rows of this V tile that belong to the sequence
         if (inside < kBK && (inside & 15) != 0) {
@@ -476,12 +565,12 @@ __global__ void __launch_bounds__(kThreads, 1)
         n += kQChunks + kVChunks;
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&bars[Smem::kPFull + x]);
+        if (lane == 0) mbar_arrive(&bars[Smem::kPFull + x_tile]);
       }
       if (!ok) break;
       n += (both - tiles) * (kQChunks + kVChunks);
       // the item's last product is complete: O is final
-      ok = mbar_wait_warp(&bars[Smem::kPvDone + x], (g - 1) & 1, p.err);
+      ok = mbar_wait_warp(&bars[Smem::kPvDone + x_tile], (g - 1) & 1, p.err);
       if (!ok) break;
       tc_fence_after();
       const float inv = l == 0.f ? 0.f : 1.f / l;
@@ -502,7 +591,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&bars[Smem::kOFree + x]);  // the next item may overwrite O
+      if (lane == 0) mbar_arrive(&bars[Smem::kOFree + x_tile]);  // the next item may overwrite O
       if (there && p.lse != nullptr)
         p.lse[tok * p.lse_tok + it.head] = l == 0.f ? -INFINITY : (m - kBias<T> + log2f(l)) * 0.6931471805599453f;
     }
