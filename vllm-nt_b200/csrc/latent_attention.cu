@@ -444,7 +444,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       fetch(first);
       const int qb = nq % L::kQBufs;
       uint64_t* const q_full = &bars[L::kQFull + qb];
-      if (nq >= L::kQBufs && !mbar_wait_warp(&bars[L::kQEmpty + qb], (nq / L::kQBufs - 1) & 1, p.err)) break;
+      if (nq >= L::kQBufs && !mbar_spin_warp(&bars[L::kQEmpty + qb], (nq / L::kQBufs - 1) & 1, p.err)) break;
       if (elected) {
         mbar_arrive_expect_tx(q_full, kChunks * rows * 128);
         const int head = pc.g % p.head_blocks * p.group_heads;
@@ -471,7 +471,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int at_page = __shfl_sync(0xffffffffu, page, i);
         const int at_group = __shfl_sync(0xffffffffu, group, i);
         const uint32_t s = nu % kRing;
-        if (nu >= kRing && !mbar_wait_warp(&bars[L::kEmpty + s], (nu / kRing - 1) & 1, p.err)) {
+        if (nu >= kRing && !mbar_spin_warp(&bars[L::kEmpty + s], (nu / kRing - 1) & 1, p.err)) {
           ok = false;
           break;
         }
@@ -488,9 +488,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     // drain the copies that may still be in flight
     for (uint32_t i = nq > L::kQBufs ? nq - L::kQBufs : 0; i < nq; ++i)
-      mbar_wait_warp(&bars[L::kQFull + i % L::kQBufs], (i / L::kQBufs) & 1, p.err);
+      mbar_spin_warp(&bars[L::kQFull + i % L::kQBufs], (i / L::kQBufs) & 1, p.err);
     for (uint32_t i = nu > kRing ? nu - kRing : 0; i < nu; ++i)
-      mbar_wait_warp(&bars[L::kFull + i % kRing], (i / kRing) & 1, p.err);
+      mbar_spin_warp(&bars[L::kFull + i % kRing], (i / kRing) & 1, p.err);
   } else if (warp == 1) {
     // -------------------------- MMA issuer: S = Q C^T --------------------------
     const uint32_t elected = elect_one();
@@ -499,15 +499,15 @@ __global__ void __launch_bounds__(kThreads, 1)
     bool ok = true;
     while (ok && walk.next(p, team, pc)) {
       const int qb = nq % L::kQBufs;
-      if (!mbar_wait_warp(&bars[L::kQFull + qb], (nq / L::kQBufs) & 1, p.err)) break;
+      if (!mbar_spin_warp(&bars[L::kQFull + qb], (nq / L::kQBufs) & 1, p.err)) break;
       const uint64_t a0 = sw128_kmajor_desc(sm + L::kQ + qb * L::kQBytes);
       for (int t = pc.t0; t < pc.t1; ++t, ++g) {
         const int s = g & 1;
         // the softmax has read this buffer's scores of two tiles ago
-        if (g >= 2) ok = mbar_wait_warp(&bars[L::kSFree + s], (g / 2 - 1) & 1, p.err);
+        if (g >= 2) ok = mbar_spin_warp(&bars[L::kSFree + s], (g / 2 - 1) & 1, p.err);
         if (pc.valid(t) > 0) {
           for (int i = 0; i < kTileUnits && ok; ++i)
-            ok = mbar_wait_warp(&bars[L::kFull + (nu + i) % kRing], ((nu + i) / kRing) & 1, p.err);
+            ok = mbar_spin_warp(&bars[L::kFull + (nu + i) % kRing], ((nu + i) / kRing) & 1, p.err);
           if (!ok) break;
           tc_fence_after();
           const uint64_t b0 = ring_desc(sm + L::kKv + nu % kRing * kUnitBytes);
@@ -527,7 +527,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     // every issued MMA completes before TMEM may be released
     commit_elected(&bars[L::kMmaDone], elected);
-    mbar_wait_warp(&bars[L::kMmaDone], 0, p.err);
+    mbar_spin_warp(&bars[L::kMmaDone], 0, p.err);
   } else if (warp == 2) {
     // ------------------------ MMA issuer: O^T += C^T P^T ------------------------
     const uint32_t elected = elect_one();
@@ -538,8 +538,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     while (ok && walk.next(p, team, pc)) {
       for (int t = pc.t0; t < pc.t1; ++t, ++g) {
         // the first product of a piece overwrites O^T: the one before has been written out
-        ok = mbar_wait_warp(&bars[L::kPFull], g & 1, p.err) &&
-             (t > pc.t0 || pieces == 0 || mbar_wait_warp(&bars[L::kOFree], (pieces - 1) & 1, p.err));
+        ok = mbar_spin_warp(&bars[L::kPFull], g & 1, p.err) &&
+             (t > pc.t0 || pieces == 0 || mbar_spin_warp(&bars[L::kOFree], (pieces - 1) & 1, p.err));
         if (!ok) break;
         const int valid = pc.valid(t);
         if (valid > 0) {
@@ -563,7 +563,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       ++pieces;
     }
     commit_elected(&bars[L::kMmaDone], elected);
-    mbar_wait_warp(&bars[L::kMmaDone], 0, p.err);
+    mbar_spin_warp(&bars[L::kMmaDone], 0, p.err);
   } else if (warp >= kFirstSmWarp) {
     // ------------------------------ softmax + output ------------------------------
     // The M = 64 product leaves row r in TMEM lane 32 (r / 16) + r % 16: warp `quad` has rows
@@ -601,7 +601,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       for (int t = pc.t0; t < pc.t1; ++t, ++g) {
         const int s = g & 1;
         const int valid = pc.valid(t);
-        bad = bad || !mbar_wait_warp(&bars[L::kSFull + s], (g / 2) & 1, p.err);
+        bad = bad || !mbar_spin_warp(&bars[L::kSFull + s], (g / 2) & 1, p.err);
         tc_fence_after();
         float x[32];
         float alpha[2] = {1.f, 1.f};
@@ -671,7 +671,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
         }
         // P and O^T are free once the product of the tile before is complete
-        if (g >= 1) bad = bad || !mbar_wait_warp(&bars[L::kPvDone], (g - 1) & 1, p.err);
+        if (g >= 1) bad = bad || !mbar_spin_warp(&bars[L::kPvDone], (g - 1) & 1, p.err);
         if (news && t > pc.t0) {
           tc_fence_after();
 #pragma unroll 1
@@ -718,7 +718,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       if (left) break;
       // O^T is final once the piece's last product is complete
-      bad = bad || !mbar_wait_warp(&bars[L::kPvDone], (g - 1) & 1, p.err);
+      bad = bad || !mbar_spin_warp(&bars[L::kPvDone], (g - 1) & 1, p.err);
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const int row = r0 + 8 * h;

@@ -16,7 +16,7 @@
 //   warp 10         TMA: Q tiles and a ring of eight 16 KB chunks (128 rows x 64 columns) that
 //                   holds K_j (3), V_j (2), K_j+1 (3).
 // While one tile's softmax runs the tensor core works for the other.  TMEM: S_A, S_B, O_A, O_B,
-// 128 columns each.  Items are dealt round robin, a sequence's last (longest) rows first.
+// 128 columns each.  Items are dealt to and fro over the CTAs, a sequence's last (longest) rows first.
 // Bound: tensor core, 2 * 320 operations a visible (query, key) pair.
 #include <algorithm>
 
@@ -36,8 +36,6 @@ constexpr int kRing = 8;
 constexpr int kThreads = 384;
 constexpr int kSWarp = 8, kPvWarp = 9, kTmaWarp = 10, kAllocWarp = 11;
 constexpr float kRescaleLog2 = 8.0f;
-// of every kEmulateOf pairs of weights kEmulated are taken on the FMA pipe
-constexpr int kEmulateOf = 4, kEmulated = 1;
 // registers: launched with 168 a thread, the two softmax warpgroups draw what the third gives up
 constexpr int kSoftmaxRegs = 208, kIssueRegs = 88;
 static_assert(256 * kSoftmaxRegs + 128 * kIssueRegs <= 384 * 168, "register split");
@@ -78,9 +76,9 @@ struct Item {
 // Walks a CTA's items (every role walks the same).  A warp holds 32 sequences' item counts at a
 // time and steps through the list as the item number grows.
 struct Walk {
-  int base;        // first sequence of the 32 held
-  int64_t before;  // items of the sequences before them
-  int64_t upto;    // this lane's inclusive count within the 32
+  int base;    // first sequence of the 32 held
+  int before;  // items of the sequences before them
+  int upto;    // this lane's inclusive count within the 32
   int q_begin, q_len, k_begin, ctx;
 
   __device__ __forceinline__ void load(const PrefillParams& p, int first) {
@@ -98,10 +96,10 @@ struct Walk {
         q_begin = q_len = k_begin = ctx = 0;
       }
     }
-    upto = int64_t((q_len + kItemRows - 1) / kItemRows) * p.num_heads;
+    upto = (q_len + kItemRows - 1) / kItemRows * p.num_heads;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const int64_t y = __shfl_up_sync(0xffffffffu, upto, o);
+      const int y = __shfl_up_sync(0xffffffffu, upto, o);
       if (lane >= o) upto += y;
     }
   }
@@ -112,9 +110,9 @@ struct Walk {
   }
 
   // item w (growing from call to call); false past the last one
-  __device__ __forceinline__ bool get(const PrefillParams& p, int64_t w, Item& it) {
+  __device__ __forceinline__ bool get(const PrefillParams& p, int w, Item& it) {
     for (;;) {
-      const int64_t all = __shfl_sync(0xffffffffu, upto, 31);
+      const int all = __shfl_sync(0xffffffffu, upto, 31);
       if (w < before + all) break;
       if (base + 32 >= p.num_seqs) return false;
       before += all;
@@ -122,14 +120,15 @@ struct Walk {
     }
     const unsigned past = __ballot_sync(0xffffffffu, w < before + upto);
     const int at = __ffs(past) - 1;
-    const int64_t prior = at > 0 ? __shfl_sync(0xffffffffu, upto, at - 1) : 0;
+    const int below = __shfl_sync(0xffffffffu, upto, at > 0 ? at - 1 : 0);
+    const int prior = at > 0 ? below : 0;
     it.q_begin = __shfl_sync(0xffffffffu, q_begin, at);
     it.q_len = __shfl_sync(0xffffffffu, q_len, at);
     it.k_begin = __shfl_sync(0xffffffffu, k_begin, at);
     it.ctx = __shfl_sync(0xffffffffu, ctx, at);
-    const int64_t i = w - before - prior;
-    const int block = int(i / p.num_heads);
-    it.head = int(i - int64_t(block) * p.num_heads);
+    const int i = w - before - prior;
+    const int block = i / p.num_heads;
+    it.head = i - block * p.num_heads;
     const int blocks = (it.q_len + kItemRows - 1) / kItemRows;
     it.q0 = (blocks - 1 - block) * kItemRows;
 #pragma unroll
@@ -151,6 +150,13 @@ __device__ __forceinline__ void tmem_st_16(uint32_t taddr, const uint32_t (&r)[1
       "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
       "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
       : "memory");
+}
+
+// A CTA's k-th item.  Rounds go over the CTAs to and fro: within a sequence items shrink, and dealt
+// in one direction the first CTA would have the larger item of every round (8192 tokens of 32
+// heads: 14% over the mean, so 2%).
+__device__ __forceinline__ int item_of(int k) {
+  return k * int(gridDim.x) + int((k & 1) ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
 }
 
 __device__ __forceinline__ float hw_exp2(float x) {
@@ -199,41 +205,6 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
   return r;
 }
-__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
-  uint64_t r;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
-__device__ __forceinline__ float max_nan(float a, float b) {
-  float r;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
-  return r;
-}
-
-// 2^y of two values on the FMA pipe: y = n + f with n whole and |f| <= 1/2, 2^f by a polynomial of
-// degree 5 (least squares of the relative error with the largest errors reweighted, the constant
-// term 1: off by 1.7e-7 in fp32), times 2^n from n's bits.  The hardware's exponentials take 8 cycles
-// a warp, 2048 of the 2560 that the tensor core needs for a pair of tiles; these are for the share
-// of them that the FMA pipe has room for.  y <= 127; below -126.5, -inf included, the result is 0;
-// a NaN stays one.
-__device__ __forceinline__ void fma_exp2(uint64_t y, float& a, float& b) {
-  float y0, y1;
-  unpack2f(y, y0, y1);
-  y = pack2f(max_nan(y0, -127.f), max_nan(y1, -127.f));
-  const float big = 12582912.f + 127.f;  // 1.5 * 2^23: the sum's low bits are n + 127
-  const uint64_t t = add2(y, pack2f(big, big));
-  const uint64_t f = add2(y, mul2(add2(t, pack2f(-big, -big)), pack2f(-1.f, -1.f)));
-  uint64_t q = fma2(f, pack2f(0.001326472731307149f, 0.001326472731307149f), pack2f(0.009671512991189957f, 0.009671512991189957f));
-  q = fma2(q, f, pack2f(0.05550733581185341f, 0.05550733581185341f));
-  q = fma2(q, f, pack2f(0.24022242426872253f, 0.24022242426872253f));
-  q = fma2(q, f, pack2f(0.6931470036506653f, 0.6931470036506653f));
-  q = fma2(q, f, pack2f(1.f, 1.f));
-  float t0, t1;
-  unpack2f(t, t0, t1);
-  q = mul2(q, pack2f(__uint_as_float(__float_as_uint(t0) << 23), __uint_as_float(__float_as_uint(t1) << 23)));
-  unpack2f(q, a, b);
-}
-
 // The running maximum is subtracted less kBias: fp16 weights then span 2^7 .. 2^15 at the
 // row's largest score and reach 2^-31 of it before they vanish (bf16 has fp32's range).
 template <typename T>
@@ -296,7 +267,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     uint32_t nq[2] = {0, 0};  // Q tiles loaded
     uint32_t n = 0;           // ring chunks loaded
     bool ok = true;
-    for (int64_t w = blockIdx.x; ok && walk.get(p, w, it); w += gridDim.x) {
+    for (int k = 0; ok && walk.get(p, item_of(k), it); ++k) {
       auto load_q = [&](int x) {
         if (!ok || it.tiles[x] == 0) return;
         uint64_t* const full = &bars[Smem::kQFull + x];
@@ -347,9 +318,12 @@ __global__ void __launch_bounds__(kThreads, 1)
     uint32_t nq[2] = {0, 0};
     uint32_t n = 0;  // ring chunks passed (V's among them)
     bool ok = true;
-    for (int64_t w = blockIdx.x; ok && walk.get(p, w, it); w += gridDim.x) {
+    for (int k = 0; ok && walk.get(p, item_of(k), it); ++k) {
       const int tiles = max(it.tiles[0], it.tiles[1]);
       for (int j = 0; ok && j < tiles; ++j, n += kQChunks + kVChunks) {
+        // what is usually there comes first: a wait that is already over costs over 100 cycles too
+        for (int c = 0; c < kQChunks && ok; ++c)
+          ok = mbar_wait_warp(&bars[Smem::kFull + (n + c) % kRing], ((n + c) / kRing) & 1, p.err);
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
           if (!ok || j >= it.tiles[x]) continue;
@@ -357,21 +331,19 @@ __global__ void __launch_bounds__(kThreads, 1)
           // the buffer's weights of the tile before have been used up
           ok = (j > 0 || mbar_wait_warp(&bars[Smem::kQFull + x], nq[x] & 1, p.err)) &&
                (ns[x] == 0 || mbar_wait_warp(&bars[Smem::kPvDone + x], (ns[x] - 1) & 1, p.err));
+          if (!ok) continue;
+          tc_fence_after();
           const uint64_t a0 = sw128_kmajor_desc(sm + Smem::kQ + x * kQChunks * kChunkBytes);
           const uint64_t b0 = sw128_kmajor_desc(sm + Smem::kKv);
 #pragma unroll
           for (int c = 0; c < kQChunks; ++c) {
             const uint32_t s = (n + c) % kRing;
-            ok = ok && mbar_wait_warp(&bars[Smem::kFull + s], ((n + c) / kRing) & 1, p.err);
-            if (!ok) break;
-            tc_fence_after();
 #pragma unroll
             for (int k = 0; k < 4; ++k)
               umma_elected(tmem + x * kBK, a0 + c * (kChunkBytes >> 4) + 2 * k, b0 + s * (kChunkBytes >> 4) + 2 * k, idesc,
                            (c | k) ? 1u : 0u, elected);
             if (last_user) commit_elected(&bars[Smem::kEmpty + s], elected);
           }
-          if (!ok) continue;
           commit_elected(&bars[Smem::kSFull + x], elected);
           ++ns[x];
           if (j + 1 == it.tiles[x]) {
@@ -394,21 +366,21 @@ __global__ void __launch_bounds__(kThreads, 1)
     uint32_t items[2] = {0, 0};  // outputs begun
     uint32_t n = 0;
     bool ok = true;
-    for (int64_t w = blockIdx.x; ok && walk.get(p, w, it); w += gridDim.x) {
+    for (int k = 0; ok && walk.get(p, item_of(k), it); ++k) {
       const int tiles = max(it.tiles[0], it.tiles[1]);
       for (int j = 0; ok && j < tiles; ++j, n += kQChunks + kVChunks) {
         const int steps = (min(it.ctx - j * kBK, kBK) + 15) / 16;
         const uint32_t s0 = (n + kQChunks) % kRing, s1 = (n + kQChunks + 1) % kRing;
         const uint64_t v0 = sw128_mnmajor_desc(sm + Smem::kKv + s0 * kChunkBytes, kChunkBytes);
         const uint64_t v1 = sw128_mnmajor_desc(sm + Smem::kKv + s1 * kChunkBytes, kChunkBytes);
+        ok = mbar_wait_warp(&bars[Smem::kFull + s0], ((n + kQChunks) / kRing) & 1, p.err) &&
+             mbar_wait_warp(&bars[Smem::kFull + s1], ((n + kQChunks + 1) / kRing) & 1, p.err);
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
           if (!ok || j >= it.tiles[x]) continue;
           const bool last_user = x == 1 || j >= it.tiles[1];
-          ok = mbar_wait_warp(&bars[Smem::kPFull + x], np[x] & 1, p.err) &&
-               (j > 0 || items[x] == 0 || mbar_wait_warp(&bars[Smem::kOFree + x], (items[x] - 1) & 1, p.err)) &&
-               mbar_wait_warp(&bars[Smem::kFull + s0], ((n + kQChunks) / kRing) & 1, p.err) &&
-               mbar_wait_warp(&bars[Smem::kFull + s1], ((n + kQChunks + 1) / kRing) & 1, p.err);
+          ok = (j > 0 || items[x] == 0 || mbar_wait_warp(&bars[Smem::kOFree + x], (items[x] - 1) & 1, p.err)) &&
+               mbar_wait_warp(&bars[Smem::kPFull + x], np[x] & 1, p.err);
           if (!ok) continue;
           tc_fence_after();
           const uint32_t o_tmem = tmem + kTmemO + x * kV, p_tmem = tmem + x * kBK;
@@ -448,24 +420,13 @@ __global__ void __launch_bounds__(kThreads, 1)
     uint32_t g = 0;  // key tiles done
     uint32_t n = 0;  // ring chunks passed
     bool ok = true;
-    for (int64_t w = blockIdx.x; ok && walk.get(p, w, it); w += gridDim.x) {
-      const int qi = it.q0 + x_tile * kBQ + r;
-      const bool there = r < it.rows[x_tile];
-      const int64_t tok = it.q_begin + qi;
-      T* const orow = static_cast<T*>(p.out) + tok * p.o_tok + int64_t(it.head) * p.o_head;
-      const int tiles = it.tiles[x_tile];
-      const int both = max(it.tiles[0], it.tiles[1]);
-      if (tiles == 0) {  // no visible key: zero rows, as for an empty softmax
-        if (there) {
-#pragma unroll
-          for (int c = 0; c < kV / 8; ++c) reinterpret_cast<uint4*>(orow)[c] = make_uint4(0u, 0u, 0u, 0u);
-          if (p.lse != nullptr) p.lse[tok * p.lse_tok + it.head] = -INFINITY;
-        }
-        n += both * (kQChunks + kVChunks);
-        continue;
-      }
+    for (int k = 0; ok && walk.get(p, item_of(k), it); ++k) {
+      const int tiles = x_tile == 0 ? it.tiles[0] : it.tiles[1];
       // this row sees keys [0, limit)
-      const int limit = !there ? 0 : p.causal ? min(max(it.ctx - it.q_len + qi + 1, 0), it.ctx) : it.ctx;
+      const int ctx = it.ctx;
+      const int limit = r >= (x_tile == 0 ? it.rows[0] : it.rows[1]) ? 0
+                        : p.causal ? min(max(ctx - it.q_len + it.q0 + x_tile * kBQ + r + 1, 0), ctx)
+                                   : ctx;
       float m = -INFINITY, l = 0.f;
       for (int j = 0; j < tiles; ++j, ++g) {
         if (!mbar_wait_warp(&bars[Smem::kSFull + x_tile], g & 1, p.err)) {
@@ -528,13 +489,9 @@ __global__ void __launch_bounds__(kThreads, 1)
           for (int i = 0; i < 16; ++i) {
             const uint64_t y = fma2(pack2f(__uint_as_float(x[c][2 * i]), __uint_as_float(x[c][2 * i + 1])), scale2, minus_m);
             float e0, e1;
-            if (i % kEmulateOf >= kEmulateOf - kEmulated) {
-              fma_exp2(y, e0, e1);
-            } else {
-              unpack2f(y, e0, e1);
-              e0 = hw_exp2(e0);
-              e1 = hw_exp2(e1);
-            }
+            unpack2f(y, e0, e1);
+            e0 = hw_exp2(e0);
+            e1 = hw_exp2(e1);
             l2[i & 1] = add2(l2[i & 1], pack2f(e0, e1));
             Pair<T>::store(reinterpret_cast<T*>(&pk[i]), e0, e1);
           }
@@ -546,7 +503,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           l += a + b;
         }
         asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
-        const int inside = it.ctx - j * kBK;  // rows of this V tile that belong to the sequence
+        const int inside = ctx - j * kBK;  // rows of this V tile that belong to the sequence
         if (inside < kBK && (inside & 15) != 0) {
           // rows behind the sequence, up to the product's next step of 16, are another's: zeroed,
           // so that a weight of 0 never meets a non-finite value
@@ -568,7 +525,19 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (lane == 0) mbar_arrive(&bars[Smem::kPFull + x_tile]);
       }
       if (!ok) break;
-      n += (both - tiles) * (kQChunks + kVChunks);
+      walk.get(p, item_of(k), it);  // (again, rather than hold it through the tiles)
+      n += (max(it.tiles[0], it.tiles[1]) - tiles) * (kQChunks + kVChunks);
+      const bool there = r < (x_tile == 0 ? it.rows[0] : it.rows[1]);
+      const int64_t tok = it.q_begin + it.q0 + x_tile * kBQ + r;
+      T* const orow = static_cast<T*>(p.out) + tok * p.o_tok + int64_t(it.head) * p.o_head;
+      if (tiles == 0) {  // no visible key: zero rows, as for an empty softmax
+        if (there) {
+#pragma unroll
+          for (int c = 0; c < kV / 8; ++c) reinterpret_cast<uint4*>(orow)[c] = make_uint4(0u, 0u, 0u, 0u);
+          if (p.lse != nullptr) p.lse[tok * p.lse_tok + it.head] = -INFINITY;
+        }
+        continue;
+      }
       // the item's last product is complete: O is final
       ok = mbar_wait_warp(&bars[Smem::kPvDone + x_tile], (g - 1) & 1, p.err);
       if (!ok) break;
@@ -658,7 +627,7 @@ extern "C" int ntb200_latent_attention_prefill(
   if (!(scale > 0.f))
     return fail(NTB200_ERR_INVALID_ARGUMENT, "latent_attention_prefill: scale must be positive");
   if (num_seqs == 0 || num_q_tokens == 0 || max_query_len == 0) return NTB200_OK;
-  if (num_seqs > 0x7fffffff - 32 || num_q_tokens > 0x7fffffff || num_k_tokens > 0x7fffffff || num_heads > 65535)
+  if (ceil_div(num_q_tokens, kItemRows) + num_seqs > (0x7fffffff - 1024) / num_heads || num_q_tokens > 0x7fffffff || num_k_tokens > 0x7fffffff || num_heads > 65535)
     return fail(NTB200_ERR_UNSUPPORTED_SHAPE, "latent_attention_prefill: sizes beyond the launch limits");
   if (!out || !query || !cu_seqlens_q || !cu_seqlens_k || (num_k_tokens > 0 && (!k_nope || !k_rope || !value)))
     return fail(NTB200_ERR_INVALID_ARGUMENT, "latent_attention_prefill: null pointer");
