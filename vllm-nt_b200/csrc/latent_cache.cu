@@ -6,8 +6,8 @@
 // Statistics, products and rotations are fp32; y and the rotated values are rounded once.
 //
 // Warps take units: unit 0 of a token is its latent row and key (one warp holds the row in
-// registers, so it is read once and no barrier is needed), the others are 128 vectors of its
-// query heads each.  HBM-bound for prefill batches, one launch's latency for decode.
+// registers, so it is read once and no barrier is needed), the others are a few vectors a lane
+// of its query heads.  HBM-bound for prefill batches, one launch's latency for decode.
 #include "common.cuh"
 #include "rope_layout.cuh"
 
@@ -38,8 +38,8 @@ template <typename T, typename C, bool INTERLEAVED>
 __global__ void __launch_bounds__(kThreads)
     latent_store_kernel(T* __restrict__ q, const T* latent, T* __restrict__ key, const T* __restrict__ weight,
                         const C* __restrict__ table, T* __restrict__ cache, T* latent_out, const StoreParams p) {
-  constexpr int kUnit = 32 * kRotItems;
   const int lane = threadIdx.x & 31;
+  constexpr int kUnit = 32 * kRotItems;
   const int q_vecs = p.num_heads * rot_vectors<kVec, INTERLEAVED>(p.rope_dim);
   const int units = 1 + (q_vecs + kUnit - 1) / kUnit;
   const int64_t u = int64_t(blockIdx.x) * (kThreads / 32) + (threadIdx.x >> 5);
@@ -59,7 +59,7 @@ __global__ void __launch_bounds__(kThreads)
   };
   if (unit > 0) {
     const TokenHeads<T> heads = {q + t * p.q_tok, nullptr, p.num_heads, 0, p.q_head, 0};
-    rotate_unit<T, C, kVec, INTERLEAVED>(heads, (unit - 1) * kUnit, p.rope_dim, row);
+    rotate_unit<T, C, kVec, INTERLEAVED, kRotItems>(heads, (unit - 1) * kUnit, p.rope_dim, row);
     return;
   }
 

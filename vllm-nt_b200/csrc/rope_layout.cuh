@@ -11,8 +11,10 @@
 namespace ntb200 {
 namespace {
 
-// Up to kRotItems vectors a lane, loaded together: 4 x 16 bytes x 32 lanes keep 2 KB a warp in
-// flight, which with 64 warps an SM is several times what HBM latency needs.
+// Vectors a lane of a prefill-sized call takes, all loaded before the first is rotated.  Consecutive
+// warps take consecutive vectors of a token, so that what is in flight lies close together in DRAM:
+// a warp that walked a whole token with the same bytes in flight was slower (8191 tokens of 128
+// heads in the store: 60 us so, 94 us walking; 78 us with 2 vectors, 68 with 6, 85 with 8).
 constexpr int kRotItems = 4;
 
 // N table entries as fp32, in 16-byte (or narrower) loads
@@ -39,6 +41,19 @@ struct RotItem {
   __device__ __forceinline__ void load(const T* p, int half) {
     a = *reinterpret_cast<const V*>(p);
     if constexpr (!INTERLEAVED) b = *reinterpret_cast<const V*>(p + half);
+  }
+  // Keeps the vectors as they were loaded until here: converted as soon as they arrive, four items
+  // of bf16 held 116 registers where they need 60.
+  __device__ __forceinline__ void pin() {
+    pin(a);
+    if constexpr (!INTERLEAVED) pin(b);
+  }
+  static __device__ __forceinline__ void pin(V& v) {
+    if constexpr (sizeof(V) % 4 == 0) {
+      uint32_t* const w = reinterpret_cast<uint32_t*>(&v);
+#pragma unroll
+      for (int i = 0; i < int(sizeof(V) / 4); ++i) asm volatile("" : "+r"(w[i]));
+    }
   }
   __device__ __forceinline__ void rotate(const float (&c)[kPairs], const float (&s)[kPairs]) {
     float x[VEC], y[VEC];
@@ -88,44 +103,44 @@ struct TokenHeads {
   }
 };
 
-// Rotates items [first + 32 j + lane] of a token, j < kRotItems, in place.  `row()` gives the
-// token's table row after the heads' loads have been issued, or null to leave them untouched.
-template <typename T, typename C, int VEC, bool INTERLEAVED, typename Row>
+// Rotates vectors first + lane + 32 j, j < ITEMS, of a token in place.  `row()` gives the token's
+// table row after the loads have been issued, or null to leave the heads untouched.
+template <typename T, typename C, int VEC, bool INTERLEAVED, int ITEMS, typename Row>
 __device__ __forceinline__ void rotate_unit(const TokenHeads<T>& t, int first, int rot, Row row) {
   using Item = RotItem<T, VEC, INTERLEAVED>;
   const int half = rot / 2;
   const int per_head = rot_vectors<VEC, INTERLEAVED>(rot);
   const int total = (t.num_q + t.num_k) * per_head;
-  const int lane = threadIdx.x & 31;
-  Item item[kRotItems];
-  T* at[kRotItems];
-  int off[kRotItems];
+  // lane l's vectors all sit at one offset of their heads when the vectors a head divide 32: one
+  // table entry serves them all, and no vector needs a division
+  const bool shared = (per_head & (per_head - 1)) == 0 && per_head <= 32;
+  const int shift = 31 - __clz(per_head);
+  const int i = first + (threadIdx.x & 31);
+  Item item[ITEMS];
+  T* at[ITEMS];
+  int off[ITEMS];
 #pragma unroll
-  for (int j = 0; j < kRotItems; ++j) {
-    const int i = first + 32 * j + lane;
-    if (i < total) {
-      const int h = i / per_head;
-      off[j] = (i - h * per_head) * VEC;
-      at[j] = t.head(h) + off[j];
-      item[j].load(at[j], half);
-    }
+  for (int j = 0; j < ITEMS; ++j) {
+    const int v = i + 32 * j;
+    const int h = shared ? v >> shift : v / per_head;
+    off[j] = (v - h * per_head) * VEC;
+    at[j] = t.head(h) + off[j];
+    if (v < total) item[j].load(at[j], half);
   }
-  const C* cs = row();
+  const C* const cs = row();
   if (cs == nullptr) return;
   float c[Item::kPairs], s[Item::kPairs];
-  // lane l's items all sit at one offset of their heads when the vectors a head divide 32
-  const bool shared = 32 % per_head == 0;
 #pragma unroll
-  for (int j = 0; j < kRotItems; ++j) {
-    if (first + 32 * j + lane < total) {
-      if (j == 0 || !shared) {
-        const int o = INTERLEAVED ? off[j] / 2 : off[j];
-        load_table<C, Item::kPairs>(cs + o, c);
-        load_table<C, Item::kPairs>(cs + half + o, s);
-      }
-      item[j].rotate(c, s);
-      item[j].store(at[j], half);
+  for (int j = 0; j < ITEMS; ++j) {
+    if (i + 32 * j >= total) break;
+    if (j == 0 || !shared) {
+      const int e = INTERLEAVED ? off[j] / 2 : off[j];
+      load_table<C, Item::kPairs>(cs + e, c);
+      load_table<C, Item::kPairs>(cs + half + e, s);
     }
+    item[j].pin();
+    item[j].rotate(c, s);
+    item[j].store(at[j], half);
   }
 }
 

@@ -1,13 +1,14 @@
 // Rotary positions in both layouts, and the cos/sin table of long contexts.
 //
 // rotary_embedding: in place on the first rotary_dim elements of every query and key head,
-// read and written once; warps take (token, 128 vectors) units, so one decode token spreads
-// over as many warps as it has units and a prefill batch fills the GPU.  Bound by HBM.
+// read and written once; a warp takes a few vectors a lane of one token's heads, so that one
+// decode token spreads over many warps.  Bound by HBM.
 //
 // rope_cos_sin_cache: row p holds cos(p f_i) and sin(p f_i) of every frequency f_i.  An fp32
 // product p * f_i is off by up to 2^-24 of the angle, 0.008 rad at 128 Ki positions and more
-// beyond: the angle is formed and reduced to [-pi, pi] in fp64 and only the remainder goes to
-// fp32 (off by at most 2^-23 rad).  A thread forms its frequency once and walks rows with it.
+// beyond: a thread forms its frequency once in fp64, in turns, and walks rows with it in 64-bit
+// fixed point, where an angle is one addition (off by 2^-64 turns a row, on top of the frequency's
+// 2^-53 of the angle); only the part of a turn goes to fp32 (off by at most 2^-26 turns, 2^-23 rad).
 #include <cmath>
 
 #include "common.cuh"
@@ -18,13 +19,13 @@ namespace {
 
 constexpr int kThreads = 256;
 
-template <typename T, typename C, int VEC, bool INTERLEAVED, typename P>
+template <typename T, typename C, int VEC, bool INTERLEAVED, int ITEMS, typename P>
 __global__ void __launch_bounds__(kThreads) rotary_kernel(const P* __restrict__ positions, T* __restrict__ q,
                                                           T* __restrict__ k, const C* __restrict__ table,
                                                           int64_t num_tokens, int num_q, int num_k, int rot,
                                                           int64_t q_tok, int64_t q_head, int64_t k_tok, int64_t k_head,
                                                           int64_t table_row, int64_t table_rows, unsigned int* err) {
-  constexpr int kUnit = 32 * kRotItems;
+  constexpr int kUnit = 32 * ITEMS;
   const int total = (num_q + num_k) * rot_vectors<VEC, INTERLEAVED>(rot);
   const int units = (total + kUnit - 1) / kUnit;
   const int64_t u = int64_t(blockIdx.x) * (kThreads / 32) + (threadIdx.x >> 5);
@@ -34,7 +35,7 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(const P* __restrict__ 
   const int64_t t = u / units;
   const int first = int(u - t * units) * kUnit;
   const TokenHeads<T> heads = {q + t * q_tok, k + t * k_tok, num_q, num_k, q_head, k_head};
-  rotate_unit<T, C, VEC, INTERLEAVED>(heads, first, rot, [&]() -> const C* {
+  rotate_unit<T, C, VEC, INTERLEAVED, ITEMS>(heads, first, rot, [&]() -> const C* {
     const int64_t pos = static_cast<int64_t>(positions[t]);
     if (pos < 0 || pos >= table_rows) {  // the token stays untouched; flagged once
       if (first == 0 && (threadIdx.x & 31) == 0) raise_device_error(err, NTB200_DEVERR_INDEX_RANGE);
@@ -53,17 +54,25 @@ struct RotaryCall {
   cudaStream_t stream;
 };
 
-template <typename T, typename C, int VEC, bool INTERLEAVED, typename P>
-int launch_rotary(const RotaryCall& c) {
-  const int64_t total = (c.hq + c.hk) * rot_vectors<VEC, INTERLEAVED>(int(c.rot));
-  const int64_t units = c.tokens * ceil_div(total, 32 * kRotItems);
+template <typename T, typename C, int VEC, bool INTERLEAVED, int ITEMS, typename P>
+int launch_items(const RotaryCall& c, int64_t total) {
+  const int64_t units = c.tokens * ceil_div(total, 32 * ITEMS);
   const int64_t ctas = ceil_div(units, kThreads / 32);
-  if (total == 0) return NTB200_OK;
   if (ctas > 0x7fffffff) return fail(NTB200_ERR_UNSUPPORTED_SHAPE, "rotary_embedding: too many tokens");
-  return launch_kernel("rotary_embedding", rotary_kernel<T, C, VEC, INTERLEAVED, P>, dim3(unsigned(ctas)),
+  return launch_kernel("rotary_embedding", rotary_kernel<T, C, VEC, INTERLEAVED, ITEMS, P>, dim3(unsigned(ctas)),
                        dim3(kThreads), 0, c.stream, static_cast<const P*>(c.positions), static_cast<T*>(c.q),
                        static_cast<T*>(c.k), static_cast<const C*>(c.table), c.tokens, int(c.hq), int(c.hk),
                        int(c.rot), c.qt, c.qh, c.kt, c.kh, c.row, c.rows, device_error_word());
+}
+
+template <typename T, typename C, int VEC, bool INTERLEAVED, typename P>
+int launch_rotary(const RotaryCall& c) {
+  const int64_t total = (c.hq + c.hk) * rot_vectors<VEC, INTERLEAVED>(int(c.rot));
+  if (total == 0) return NTB200_OK;
+  // a call that leaves SMs idle is spread one vector a lane (7 tokens of 40 heads: 1.8 us against 2.2)
+  if (c.tokens * ceil_div(total, 32 * kRotItems) < int64_t(num_sms()) * 8)
+    return launch_items<T, C, VEC, INTERLEAVED, 1, P>(c, total);
+  return launch_items<T, C, VEC, INTERLEAVED, kRotItems, P>(c, total);
 }
 
 template <typename T, typename C, int VEC, bool INTERLEAVED>
@@ -102,11 +111,12 @@ int by_table(const RotaryCall& c, int table_dtype, int dtype, bool interleaved) 
 
 // ---- the table ----
 
-constexpr int kRowsPerThread = 8;
+constexpr int kMaxThreadRows = 16;
 
 struct TableParams {
   int64_t rows, first, row_stride;
   int half;
+  int thread_rows;    // rows a thread forms
   double log_step;    // ln f_{i+1} - ln f_i before scaling
   double linear;      // every frequency times this (1: unscaled)
   double ramp_lo, ramp_inv;  // yarn: share of the divided frequency = clamp((i - lo) * inv, 0, 1)
@@ -122,7 +132,7 @@ __global__ void __launch_bounds__(kThreads) cos_sin_kernel(T* __restrict__ out, 
   const int lanes = p.half < kThreads ? p.half : kThreads;  // threads along the frequencies
   const int strip = kThreads / lanes;                       // rows a CTA writes at once
   if (int(threadIdx.x) >= strip * lanes) return;
-  const int64_t row0 = int64_t(blockIdx.x) * strip * kRowsPerThread + threadIdx.x / lanes;
+  const int64_t row0 = int64_t(blockIdx.x) * strip * p.thread_rows + threadIdx.x / lanes;
   for (int i = threadIdx.x % lanes; i < p.half; i += lanes) {
     double f = exp(i * p.log_step) * p.linear;
     if (p.yarn != 0.0) {
@@ -130,16 +140,18 @@ __global__ void __launch_bounds__(kThreads) cos_sin_kernel(T* __restrict__ out, 
       f = f * p.yarn * share + f * (1.0 - share);
     }
     if (p.divisors != nullptr) f /= double(p.divisors[i]);
-#pragma unroll
-    for (int r = 0; r < kRowsPerThread; ++r) {
+    // whole turns count for nothing: the angle of a row is its number times f's part of a turn in
+    // units of 2^-64 turns, whose 64-bit product and sums drop the whole turns by themselves
+    f *= 0.15915494309189535;
+    const uint64_t unit = static_cast<uint64_t>((f - floor(f)) * 18446744073709551616.0);
+    const uint64_t step = unit * static_cast<uint64_t>(strip);
+    uint64_t phase = unit * static_cast<uint64_t>(p.first + row0);
+#pragma unroll 4
+    for (int r = 0; r < p.thread_rows; ++r, phase += step) {
       const int64_t row = row0 + int64_t(r) * strip;
       if (row >= p.rows) break;
-      const double angle = double(p.first + row) * f;
-      // minus the nearest whole number of turns, 2 pi held in two doubles
-      const double turns = rint(angle * 0.15915494309189535);
-      const double rest = fma(-turns, 2.4492935982947064e-16, fma(-turns, 6.283185307179586, angle));
       float s, c;
-      sincosf(float(rest), &s, &c);
+      sincospif(float(static_cast<int32_t>(phase >> 32)) * 4.656612873077393e-10f, &s, &c);  // half turns
       T* const o = out + row * p.row_stride;
       o[i] = Elem<T>::from_f(c * p.magnitude);
       o[p.half + i] = Elem<T>::from_f(s * p.magnitude);
@@ -147,10 +159,16 @@ __global__ void __launch_bounds__(kThreads) cos_sin_kernel(T* __restrict__ out, 
   }
 }
 
+// Rows a thread: a frequency costs about as much as 4 of them, so many for a long table (131075 x 64:
+// 11.4 us with 16, 12.9 with 8, 14.1 with 32, whose last wave is part-filled), but a short one is
+// spread over four CTAs an SM first (4096 x 128: 3.3 us with 16, 2.7 with 8).
 template <typename T>
-int launch_table(void* out, const TableParams& p, cudaStream_t stream) {
+int launch_table(void* out, TableParams p, cudaStream_t stream) {
   const int lanes = p.half < kThreads ? p.half : kThreads;
-  const int64_t ctas = ceil_div(p.rows, int64_t(kThreads / lanes) * kRowsPerThread);
+  const int strip = kThreads / lanes;
+  const int64_t per = ceil_div(p.rows, int64_t(strip) * num_sms() * 4);
+  p.thread_rows = int(per < 2 ? 2 : per > kMaxThreadRows ? kMaxThreadRows : per);
+  const int64_t ctas = ceil_div(p.rows, int64_t(strip) * p.thread_rows);
   if (ctas > 0x7fffffff) return fail(NTB200_ERR_UNSUPPORTED_SHAPE, "rope_cos_sin_cache: too many rows");
   return launch_kernel("rope_cos_sin_cache", cos_sin_kernel<T>, dim3(unsigned(ctas)), dim3(kThreads), 0, stream,
                        static_cast<T*>(out), p);

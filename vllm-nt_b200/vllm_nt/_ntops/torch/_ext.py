@@ -75,5 +75,17 @@ def ops():
     return torch.ops.ntb200
 
 
+_overloads: dict[str, object] = {}
+
+
+def overload(name: str):
+    """``torch.ops.ntb200.<name>.default``, looked up once: resolving the overload at each call
+    costs 0.6 us, a tenth of a small op's whole call."""
+    op = _overloads.get(name)
+    if op is None:
+        op = _overloads[name] = getattr(ops(), name).default
+    return op
+
+
 def loaded_paths() -> list[str]:
     return [str(LIBRARY), str(BINDING)] if _loaded else []

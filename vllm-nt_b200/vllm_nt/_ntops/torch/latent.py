@@ -6,11 +6,18 @@ from __future__ import annotations
 
 import torch
 
-from vllm_nt._ntops.torch._ext import ops
+from vllm_nt._ntops.torch._ext import ops, overload
 
 
 def _flat(t: torch.Tensor) -> torch.Tensor:
-    t = t.reshape(-1)
+    if t.dim() != 1:
+        t = t.reshape(-1)
+    return t if t.is_contiguous() else t.contiguous()
+
+
+def _int32(t: torch.Tensor) -> torch.Tensor:
+    if t.dtype != torch.int32:
+        t = t.to(torch.int32)
     return t if t.is_contiguous() else t.contiguous()
 
 
@@ -34,8 +41,8 @@ def latent_rope_and_cache(
     kv_cache[slot_mapping[t]] = [latent | key].  ``latent_out`` [T, 512] (it may be ``latent``)
     receives the normalised rows.  Tokens past ``slot_mapping.numel()`` and those with a negative
     slot (vLLM's padded rows) are not stored."""
-    ops().latent_rope_and_cache(_flat(positions), query, latent, key, norm_weight, float(eps), cos_sin_cache,
-                                bool(interleaved), kv_cache, latent_out, _flat(slot_mapping))
+    overload("latent_rope_and_cache")(_flat(positions), query, latent, key, norm_weight, eps, cos_sin_cache, interleaved,
+                                      kv_cache, latent_out, _flat(slot_mapping))
 
 
 def latent_workspace_bytes() -> int:
@@ -68,14 +75,13 @@ def latent_attention(
     ``max_query_len`` bounds the query counts (None: T), ``max_seq_len`` the lengths (None: the
     block table's capacity).  ``lse`` float32 [T, heads] receives the natural log of the
     softmax sums.  ``workspace`` may be passed to avoid an allocation per call."""
-    seq_lens = seq_lens if seq_lens.dtype == torch.int32 else seq_lens.to(torch.int32)
-    block_table = block_table if block_table.dtype == torch.int32 else block_table.to(torch.int32)
     if query_start_loc is not None:
-        qsl = query_start_loc if query_start_loc.dtype == torch.int32 else query_start_loc.to(torch.int32)
-        query_start_loc = qsl.contiguous()
-    most = q_latent.shape[0] if max_query_len is None else int(max_query_len)
-    ops().latent_attention(out, lse, q_latent, q_rope, kv_cache, query_start_loc, seq_lens.contiguous(), block_table,
-                           most, int(max_seq_len or 0), float(scale), workspace)
+        query_start_loc = _int32(query_start_loc)
+    if block_table.dtype != torch.int32:
+        block_table = block_table.to(torch.int32)
+    overload("latent_attention")(out, lse, q_latent, q_rope, kv_cache, query_start_loc, _int32(seq_lens), block_table,
+                                 q_latent.shape[0] if max_query_len is None else max_query_len, max_seq_len or 0, scale,
+                                 workspace)
     return out
 
 
@@ -98,8 +104,6 @@ def latent_attention_prefill(
     rows cu_seqlens_q[b] .. [b + 1] and cu_seqlens_k[b] .. [b + 1], causal masking aligned to the
     end of its keys.  ``lse`` float32 [Tq, heads] receives the natural log of the softmax sums,
     with which two parts of a context can be merged."""
-    cu_q = cu_seqlens_q if cu_seqlens_q.dtype == torch.int32 else cu_seqlens_q.to(torch.int32)
-    cu_k = cu_seqlens_k if cu_seqlens_k.dtype == torch.int32 else cu_seqlens_k.to(torch.int32)
-    ops().latent_attention_prefill(out, lse, query, k_nope, k_rope, value, cu_q.contiguous(), cu_k.contiguous(),
-                                   int(max_query_len), float(scale), bool(causal))
+    overload("latent_attention_prefill")(out, lse, query, k_nope, k_rope, value, _int32(cu_seqlens_q),
+                                         _int32(cu_seqlens_k), max_query_len, scale, causal)
     return out

@@ -10,7 +10,7 @@ import math
 import torch
 
 from vllm_nt._ntops import capi
-from vllm_nt._ntops.torch._ext import ops
+from vllm_nt._ntops.torch._ext import ops, overload
 
 _SCALINGS = {None: capi.ROPE_NONE, "none": capi.ROPE_NONE, "linear": capi.ROPE_LINEAR, "ntk": capi.ROPE_NTK,
              "yarn": capi.ROPE_YARN}
@@ -40,7 +40,8 @@ def rotary_embedding(
     that are a column slice (the rotary part at a head's end) are passed as the 3-D slice."""
     rot = cos_sin_cache.shape[-1] if rotary_dim is None else rotary_dim
     if interleaved or cos_sin_cache.dtype != query.dtype:
-        return _rotary_either_layout(positions, query, key, int(head_size), cos_sin_cache, int(rot), bool(interleaved))
+        _rotary_either_layout(positions, query, key, head_size, cos_sin_cache, rot, interleaved)
+        return query, key
     if (positions.is_contiguous() and cos_sin_cache.is_contiguous() and query.dim() == 2
             and query.stride(-1) == 1 and (key is None or (key.dim() == 2 and key.stride(-1) == 1))):
         # vLLM's [tokens, heads * head_size] slices of the qkv projection go straight in
@@ -57,23 +58,18 @@ def rotary_embedding(
     return query, key
 
 
-def _sliced_heads(t: torch.Tensor, num_tokens: int, head_size: int) -> torch.Tensor:
-    """[tokens, heads, head_size] of rows of heads, or of a 3-D slice as it is."""
-    if t.dim() == 3 and t.shape[0] == num_tokens and t.shape[2] == head_size and t.stride(2) == 1:
-        return t
-    return _heads(t, num_tokens, head_size)
-
-
 def _rotary_either_layout(positions, query, key, head_size, cos_sin_cache, rot, interleaved):
-    positions = positions.reshape(-1)
+    # rows of heads [tokens, heads * head_size] and [tokens, heads, head_size] slices go straight in
     if not positions.is_contiguous():
         positions = positions.contiguous()
-    n = positions.shape[0]
-    cache = cos_sin_cache if cos_sin_cache.stride(-1) == 1 else cos_sin_cache.contiguous()
-    q = _sliced_heads(query, n, head_size)
-    k = _sliced_heads(key, n, head_size) if key is not None else None
-    ops().rotary_embedding(positions, q, k, cache, head_size, rot, interleaved)
-    return query, key
+    if cos_sin_cache.stride(-1) != 1:
+        cos_sin_cache = cos_sin_cache.contiguous()
+    n = positions.numel()
+    if query.dim() > 3 or query.shape[0] != n:
+        query = _heads(query, n, head_size)
+    if key is not None and (key.dim() > 3 or key.shape[0] != n):
+        key = _heads(key, n, head_size)
+    overload("rotary_embedding")(positions, query, key, cos_sin_cache, head_size, rot, interleaved)
 
 
 def rope_cos_sin_cache(
@@ -111,9 +107,8 @@ def rope_cos_sin_cache(
         out = torch.empty(num_positions, rotary_dim, dtype=dtype, device="cuda" if device is None else device)
     elif out.dim() != 2 or out.shape[0] != num_positions:
         raise ValueError("rope_cos_sin_cache: out must be [num_positions, >= rotary_dim]")
-    ops().rope_cos_sin_cache(out, int(first_position), int(rotary_dim), float(base), _SCALINGS[scaling], float(factor),
-                             float(original_max_position or 0), float(beta_fast), float(beta_slow), float(magnitude),
-                             freq_divisors)
+    overload("rope_cos_sin_cache")(out, first_position, rotary_dim, base, _SCALINGS[scaling], factor,
+                                   original_max_position or 0, beta_fast, beta_slow, magnitude, freq_divisors)
     return out
 
 
