@@ -948,7 +948,7 @@ extern "C" int ntb200_latent_attention(
     return fail(NTB200_ERR_INVALID_ARGUMENT, "latent_attention: without query_start_loc every sequence has num_tokens / num_seqs queries");
   if (num_seqs == 0 || num_tokens == 0 || (query_start_loc != nullptr && max_query_len == 0)) return NTB200_OK;
   if (num_seqs > 0x7fffffff || num_tokens > 0x7fffffff || num_heads > 65535 || num_blocks > 0x7fffffff ||
-      max_blocks_per_seq > 0x7fffffff / block_size)
+      max_blocks_per_seq > (0x7fffffff - 1024) / block_size)
     return fail(NTB200_ERR_UNSUPPORTED_SHAPE, "latent_attention: sizes beyond the launch limits");
   if (!out || !q_latent || !q_rope || !seq_lens || (max_blocks_per_seq > 0 && (!block_tables || !kv_cache || num_blocks == 0)))
     return fail(NTB200_ERR_INVALID_ARGUMENT, "latent_attention: null pointer");

@@ -627,7 +627,9 @@ extern "C" int ntb200_latent_attention_prefill(
   if (!(scale > 0.f))
     return fail(NTB200_ERR_INVALID_ARGUMENT, "latent_attention_prefill: scale must be positive");
   if (num_seqs == 0 || num_q_tokens == 0 || max_query_len == 0) return NTB200_OK;
-  if (ceil_div(num_q_tokens, kItemRows) + num_seqs > (0x7fffffff - 1024) / num_heads || num_q_tokens > 0x7fffffff || num_k_tokens > 0x7fffffff || num_heads > 65535)
+  constexpr int64_t kMost = 0x7fffffff - 1024;  // row numbers rounded up to a tile stay 32-bit
+  if (num_heads > 65535 || num_q_tokens > kMost || num_k_tokens > kMost || num_seqs > kMost ||
+      ceil_div(num_q_tokens, kItemRows) + num_seqs > kMost / num_heads)
     return fail(NTB200_ERR_UNSUPPORTED_SHAPE, "latent_attention_prefill: sizes beyond the launch limits");
   if (!out || !query || !cu_seqlens_q || !cu_seqlens_k || (num_k_tokens > 0 && (!k_nope || !k_rope || !value)))
     return fail(NTB200_ERR_INVALID_ARGUMENT, "latent_attention_prefill: null pointer");

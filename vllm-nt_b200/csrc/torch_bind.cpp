@@ -5,6 +5,7 @@
 // c10::Error carrying the status string and detail.  There is no CPU implementation: a
 // CPU tensor reaching these ops is an error, never a silent fallback.
 #include <ATen/ATen.h>
+#include <ATen/MemoryOverlap.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/library.h>
@@ -726,6 +727,12 @@ void same_device(const at::Tensor& a, const at::Tensor& b, const char* what) {
   TORCH_CHECK(b.is_cuda() && a.device() == b.device(), "ntb200.", what, ": tensors on different devices");
 }
 
+// A tensor that is written: no two of its elements may share memory (an expanded one).
+void written(const at::Tensor& t, const char* what, const char* name) {
+  TORCH_CHECK(at::has_internal_overlap(t) != at::MemOverlap::Yes, "ntb200.", what, ": ", name,
+              " is written, its elements must not share memory");
+}
+
 int index_code(const at::Tensor& t, const char* what, const char* name) {
   TORCH_CHECK(t.scalar_type() == at::kInt || t.scalar_type() == at::kLong, "ntb200.", what, ": ", name,
               " must be int32 or int64");
@@ -744,6 +751,8 @@ void rotary_embedding(const at::Tensor& positions, at::Tensor query, const std::
               "ntb200.rotary_embedding: cos_sin_cache must be float32 or of query's dtype");
   TORCH_CHECK(rotary_dim <= cache.size(1), "ntb200.rotary_embedding: rotary_dim exceeds cos_sin_cache's rows");
   TORCH_CHECK(head_size > 0, "ntb200.rotary_embedding: head_size must be positive");
+  written(query, "rotary_embedding", "query");
+  if (key.has_value()) written(*key, "rotary_embedding", "key");
   const int64_t tokens = positions.numel();
   int64_t hq = 0, qts = 0, qhs = 0, hk = 0, kts = 0, khs = 0;
   head_geometry(query, tokens, head_size, "query", hq, qts, qhs);
@@ -768,6 +777,7 @@ void rope_cos_sin_cache(at::Tensor out, int64_t first_position, int64_t rotary_d
                         double factor, double original_max_position, double beta_fast, double beta_slow,
                         double magnitude, const std::optional<at::Tensor>& freq_divisors) {
   require_rows(out, "out");
+  written(out, "rope_cos_sin_cache", "out");
   TORCH_CHECK(rotary_dim > 0 && rotary_dim <= out.size(1), "ntb200.rope_cos_sin_cache: rotary_dim exceeds out's rows");
   const float* div = nullptr;
   if (freq_divisors.has_value()) {
@@ -800,6 +810,10 @@ void latent_rope_and_cache(const at::Tensor& positions, const std::optional<at::
   same_device(latent, cos_sin_cache, op);
   same_device(latent, kv_cache, op);
   same_device(latent, slot_mapping, op);
+  written(key, op, "key");
+  written(kv_cache, op, "kv_cache");
+  if (query.has_value()) written(*query, op, "query");
+  if (latent_out.has_value()) written(*latent_out, op, "latent_out");
   const int64_t tokens = latent.size(0), ld = latent.size(1), rd = key.size(1);
   const auto dt = latent.scalar_type();
   TORCH_CHECK(positions.is_contiguous() && positions.numel() == tokens && key.size(0) == tokens,
@@ -861,6 +875,8 @@ void latent_attention(at::Tensor out, const std::optional<at::Tensor>& lse, cons
   same_device(q_latent, kv_cache, op);
   same_device(q_latent, seq_lens, op);
   same_device(q_latent, block_table, op);
+  written(out, op, "out");
+  if (lse.has_value()) written(*lse, op, "lse");
   const auto dt = q_latent.scalar_type();
   TORCH_CHECK(q_latent.dim() == 3 && q_rope.dim() == 3 && q_latent.stride(2) == 1 && q_rope.stride(2) == 1 &&
                   q_rope.size(0) == q_latent.size(0) && q_rope.size(1) == q_latent.size(1) &&
@@ -934,6 +950,8 @@ void latent_attention_prefill(at::Tensor out, const std::optional<at::Tensor>& l
   same_device(query, value, op);
   same_device(query, cu_seqlens_q, op);
   same_device(query, cu_seqlens_k, op);
+  written(out, op, "out");
+  if (lse.has_value()) written(*lse, op, "lse");
   const auto dt = query.scalar_type();
   TORCH_CHECK(query.dim() == 3 && query.stride(2) == 1 && k_nope.dim() == 3 && k_nope.stride(2) == 1 &&
                   value.dim() == 3 && value.stride(2) == 1 && k_rope.dim() == 2 && k_rope.stride(1) == 1,

@@ -65,9 +65,9 @@ def _rotary_either_layout(positions, query, key, head_size, cos_sin_cache, rot, 
     if cos_sin_cache.stride(-1) != 1:
         cos_sin_cache = cos_sin_cache.contiguous()
     n = positions.numel()
-    if query.dim() > 3 or query.shape[0] != n:
+    if query.dim() not in (2, 3) or query.shape[0] != n or (query.dim() == 3 and query.shape[2] != head_size):
         query = _heads(query, n, head_size)
-    if key is not None and (key.dim() > 3 or key.shape[0] != n):
+    if key is not None and (key.dim() not in (2, 3) or key.shape[0] != n or (key.dim() == 3 and key.shape[2] != head_size)):
         key = _heads(key, n, head_size)
     overload("rotary_embedding")(positions, query, key, cos_sin_cache, head_size, rot, interleaved)
 
