@@ -7,19 +7,20 @@
 //
 // Persistent, one CTA per SM, 384 threads.  A work item is 256 query rows of one head, as two
 // 128-row tiles A and B that share every K and V tile (128 keys) brought in:
-//   warps 0-3, 4-7  softmax of tile A, B: one thread a row, whose 128 scores it holds in
-//                   registers (208 a thread, drawn from the issuing warps'); the running maximum
-//                   is refreshed only when it grows by over 2^8 (the output is rescaled then);
-//                   weights go back to TMEM over the scores, rounded to the type.
+//   warps 0-3, 4-7  softmax of tile A, B: one thread a row, whose 128 scores it takes into
+//                   registers at once (208 a thread, drawn from the issuing warps'), so that one
+//                   S buffer serves both tiles and the next product runs while this one's softmax
+//                   does; the running maximum is refreshed only when it grows by over 2^8 (the
+//                   output is rescaled then); weights go to TMEM, rounded to the type.
 //   warp 8          S = Q K^T of A and B in turn (tcgen05, M = N = 128, twelve steps of 16).
 //   warp 9          O += P V (P from TMEM, V as it lies, MN-major, in two halves of 64 columns).
-//   warp 10         TMA: Q tiles and a ring of eight 16 KB chunks (128 rows x 64 columns) that
-//                   holds K_j (3), V_j (2), K_j+1 (3).
-// While one tile's softmax runs the tensor core works for the other.  TMEM: S_A, S_B, O_A, O_B,
-// 128 columns each.  Items are dealt to and fro over the CTAs, a sequence's last (longest) rows first.
+//   warp 10         TMA: Q tiles and a ring of eight 16 KB chunks (128 rows x 64 columns), K_j+1
+//                   ahead of V_j, as S runs a tile ahead of P V.
+// TMEM: S 128 columns, P_A and P_B 64 each, O_A and O_B 128 each.  Items are dealt to and fro over
+// the CTAs, a sequence's last (longest) rows first.
 // Bound: tensor core, 2 * 320 operations a visible (query, key) pair.  A causal prompt of 8192
-// tokens and 32 heads takes 635 us, 1080 TFLOP/s: the chain scores (768 cycles of MMAs), softmax
-// (2000), P V (505) of two tiles leaves the tensor core 62 % busy.
+// tokens and 32 heads takes 548 us, 1255 TFLOP/s (635 us with an S buffer a tile that also held its
+// weights, which kept a tile's next product waiting for P V).
 #include <algorithm>
 
 #include "common.cuh"
@@ -42,16 +43,23 @@ constexpr float kRescaleLog2 = 8.0f;
 constexpr int kSoftmaxRegs = 208, kIssueRegs = 88;
 static_assert(256 * kSoftmaxRegs + 128 * kIssueRegs <= 384 * 168, "register split");
 constexpr uint32_t kTmemCols = 512;
-constexpr uint32_t kTmemO = 256;  // S_A, S_B at 0, 128; O_A, O_B at 256, 384
+constexpr uint32_t kTmemP = 128;  // S at 0; P_A, P_B at 128, 192
+constexpr uint32_t kTmemO = 256;  // O_A, O_B at 256, 384
+
+// Where in the ring the CTA's g-th key tile lies: its keys in chunks 5 g .. 5 g + 2, its values
+// behind the next tile's keys.  So what a chunk takes the place of is: K_g, of K_g-2's last chunk and V_g-3;
+// V_g, of K_g's first two.
+__device__ __forceinline__ uint32_t k_chunk(uint32_t g) { return g * (kQChunks + kVChunks); }
+__device__ __forceinline__ uint32_t v_chunk(uint32_t g) { return k_chunk(g + 1) + kQChunks; }
+static_assert(kQChunks == 3 && kVChunks == 2 && kRing == 8, "the ring's order");
 
 struct Smem {
   static constexpr int kQ = 0;  // [2 tiles][3 chunks]
   static constexpr int kKv = kQ + 2 * kQChunks * kChunkBytes;
   static constexpr int kBars = kKv + kRing * kChunkBytes;
-  // indexes of the mbarriers
-  static constexpr int kQFull = 0, kQEmpty = 2, kFull = 4, kEmpty = kFull + kRing, kSFull = kEmpty + kRing,
-                       kPFull = kSFull + 2, kPvDone = kPFull + 2, kOFree = kPvDone + 2, kMmaDone = kOFree + 2,
-                       kNumBars = kMmaDone + 1;
+  // indexes of the mbarriers: one of each for tile A and B, or for even and odd key tiles
+  static constexpr int kQFull = 0, kQEmpty = 2, kKFull = 4, kKEmpty = 6, kVFull = 8, kVEmpty = 10, kSFull = 12,
+                       kPFull = 14, kPvDone = 16, kOFree = 18, kSFree = 20, kMmaDone = 21, kNumBars = 22;
   static constexpr int kTmemBase = kBars + 8 * kNumBars;
   static constexpr int kBytes = kTmemBase + 16;
 };
@@ -230,12 +238,16 @@ __global__ void __launch_bounds__(kThreads, 1)
     for (int i = 0; i < 2; ++i) {
       mbar_init(&bars[Smem::kQFull + i], 1);
       mbar_init(&bars[Smem::kQEmpty + i], 1);
+      mbar_init(&bars[Smem::kKFull + i], 1);
+      mbar_init(&bars[Smem::kKEmpty + i], 1);
+      mbar_init(&bars[Smem::kVFull + i], 1);
+      mbar_init(&bars[Smem::kVEmpty + i], 1);
       mbar_init(&bars[Smem::kSFull + i], 1);
       mbar_init(&bars[Smem::kPFull + i], 4);  // one arrive a softmax warp
       mbar_init(&bars[Smem::kPvDone + i], 1);
       mbar_init(&bars[Smem::kOFree + i], 4);
     }
-    for (int i = 0; i < kRing; ++i) mbar_init(&bars[Smem::kFull + i], 1), mbar_init(&bars[Smem::kEmpty + i], 1);
+    mbar_init(&bars[Smem::kSFree], 4);
     mbar_init(&bars[Smem::kMmaDone], 2);
     fence_mbar_init();
   }
@@ -267,8 +279,24 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     __syncwarp();
     uint32_t nq[2] = {0, 0};  // Q tiles loaded
-    uint32_t n = 0;           // ring chunks loaded
+    uint32_t nk = 0, nv = 0;  // key tiles loaded, value tiles loaded (one behind)
+    int v_head = 0, v_row = 0;  // of value tile nv
     bool ok = true;
+    auto load_v = [&]() {
+      if (!ok || nv == nk) return;
+      // its keys have been used
+      ok = mbar_wait_warp(&bars[Smem::kKEmpty + (nv & 1)], (nv / 2) & 1, p.err);
+      if (!ok) return;
+      if (elected) {
+        uint64_t* const full = &bars[Smem::kVFull + (nv & 1)];
+        mbar_arrive_expect_tx(full, kVChunks * kChunkBytes);
+        for (int c = 0; c < kVChunks; ++c)
+          tma_load_3d(sm + Smem::kKv + (v_chunk(nv) + c) % kRing * kChunkBytes, &v_map, c * 64, v_head, v_row,
+                      smem_u32(full));
+      }
+      __syncwarp();
+      ++nv;
+    };
     for (int k = 0; ok && walk.get(p, item_of(k), it); ++k) {
       auto load_q = [&](int x) {
         if (!ok || it.tiles[x] == 0) return;
@@ -288,66 +316,65 @@ __global__ void __launch_bounds__(kThreads, 1)
       load_q(0);
       for (int j = 0; ok && j < tiles; ++j) {
         const int row = it.k_begin + j * kBK;
-#pragma unroll 1
-        for (int c = 0; ok && c < kQChunks + kVChunks; ++c) {
-          const uint32_t s = n % kRing;
-          if (n >= kRing) ok = mbar_wait_warp(&bars[Smem::kEmpty + s], (n / kRing - 1) & 1, p.err);
-          if (!ok) break;
-          if (elected) {
-            uint64_t* const full = &bars[Smem::kFull + s];
-            const uint32_t dst = sm + Smem::kKv + s * kChunkBytes;
-            mbar_arrive_expect_tx(full, kChunkBytes);
+        if (nk >= 3) ok = mbar_wait_warp(&bars[Smem::kVEmpty + ((nk - 3) & 1)], ((nk - 3) / 2) & 1, p.err);
+        if (!ok) break;
+        if (elected) {
+          uint64_t* const full = &bars[Smem::kKFull + (nk & 1)];
+          mbar_arrive_expect_tx(full, kQChunks * kChunkBytes);
+          for (int c = 0; c < kQChunks; ++c) {
+            const uint32_t dst = sm + Smem::kKv + (k_chunk(nk) + c) % kRing * kChunkBytes;
             if (c < kNope / 64) tma_load_3d(dst, &kn_map, c * 64, it.head, row, smem_u32(full));
-            else if (c < kQChunks) tma_load_2d(dst, &kr_map, 0, row, smem_u32(full));
-            else tma_load_3d(dst, &v_map, (c - kQChunks) * 64, it.head, row, smem_u32(full));
+            else tma_load_2d(dst, &kr_map, 0, row, smem_u32(full));
           }
-          __syncwarp();
-          ++n;
-          if (j == 0 && c == kQChunks - 1) load_q(1);
         }
+        __syncwarp();
+        if (j == 0) load_q(1);
+        load_v();  // of the tile before
+        ++nk;
+        v_head = it.head;
+        v_row = row;
       }
     }
+    load_v();
     // drain the copies that may still be in flight
     for (int x = 0; x < 2; ++x)
       if (nq[x] > 0) mbar_wait_warp(&bars[Smem::kQFull + x], (nq[x] - 1) & 1, p.err);
-    for (uint32_t i = n > kRing ? n - kRing : 0; i < n; ++i)
-      mbar_wait_warp(&bars[Smem::kFull + i % kRing], (i / kRing) & 1, p.err);
+    for (uint32_t g = nk > 2 ? nk - 2 : 0; g < nk; ++g) mbar_wait_warp(&bars[Smem::kKFull + (g & 1)], (g / 2) & 1, p.err);
+    for (uint32_t g = nv > 2 ? nv - 2 : 0; g < nv; ++g) mbar_wait_warp(&bars[Smem::kVFull + (g & 1)], (g / 2) & 1, p.err);
   } else if (warp == kSWarp) {
     // -------------------------- MMA issuer: S = Q K^T --------------------------
     const uint32_t elected = elect_one();
     const uint32_t idesc = make_idesc(std::is_same<T, __nv_bfloat16>::value, kBQ, kBK);
-    uint32_t ns[2] = {0, 0};  // products issued a tile
     uint32_t nq[2] = {0, 0};
-    uint32_t n = 0;  // ring chunks passed (V's among them)
+    uint32_t g = 0, ns = 0;  // key tiles passed, products issued
     bool ok = true;
     for (int k = 0; ok && walk.get(p, item_of(k), it); ++k) {
       const int tiles = max(it.tiles[0], it.tiles[1]);
-      for (int j = 0; ok && j < tiles; ++j, n += kQChunks + kVChunks) {
+      for (int j = 0; ok && j < tiles; ++j, ++g) {
         // what is usually there comes first: a wait that is already over costs over 100 cycles too
-        for (int c = 0; c < kQChunks && ok; ++c)
-          ok = mbar_wait_warp(&bars[Smem::kFull + (n + c) % kRing], ((n + c) / kRing) & 1, p.err);
+        ok = mbar_wait_warp(&bars[Smem::kKFull + (g & 1)], (g / 2) & 1, p.err);
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
           if (!ok || j >= it.tiles[x]) continue;
           const bool last_user = x == 1 || j >= it.tiles[1];
-          // the buffer's weights of the tile before have been used up
+          // the product before is in its warps' registers
           ok = (j > 0 || mbar_wait_warp(&bars[Smem::kQFull + x], nq[x] & 1, p.err)) &&
-               (ns[x] == 0 || mbar_wait_warp(&bars[Smem::kPvDone + x], (ns[x] - 1) & 1, p.err));
+               (ns == 0 || mbar_wait_warp(&bars[Smem::kSFree], (ns - 1) & 1, p.err));
           if (!ok) continue;
           tc_fence_after();
           const uint64_t a0 = sw128_kmajor_desc(sm + Smem::kQ + x * kQChunks * kChunkBytes);
           const uint64_t b0 = sw128_kmajor_desc(sm + Smem::kKv);
 #pragma unroll
           for (int c = 0; c < kQChunks; ++c) {
-            const uint32_t s = (n + c) % kRing;
+            const uint32_t s = (k_chunk(g) + c) % kRing;
 #pragma unroll
             for (int k = 0; k < 4; ++k)
-              umma_elected(tmem + x * kBK, a0 + c * (kChunkBytes >> 4) + 2 * k, b0 + s * (kChunkBytes >> 4) + 2 * k, idesc,
+              umma_elected(tmem, a0 + c * (kChunkBytes >> 4) + 2 * k, b0 + s * (kChunkBytes >> 4) + 2 * k, idesc,
                            (c | k) ? 1u : 0u, elected);
-            if (last_user) commit_elected(&bars[Smem::kEmpty + s], elected);
           }
           commit_elected(&bars[Smem::kSFull + x], elected);
-          ++ns[x];
+          if (last_user) commit_elected(&bars[Smem::kKEmpty + (g & 1)], elected);
+          ++ns;
           if (j + 1 == it.tiles[x]) {
             commit_elected(&bars[Smem::kQEmpty + x], elected);
             ++nq[x];
@@ -366,17 +393,26 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t idesc_half = make_idesc(kBf16, kBQ, 64) | (1u << 16);  // one chunk of it
     uint32_t np[2] = {0, 0};     // products issued a tile
     uint32_t items[2] = {0, 0};  // outputs begun
-    uint32_t n = 0;
+    uint32_t g = 0;              // key tiles passed
     bool ok = true;
     for (int k = 0; ok && walk.get(p, item_of(k), it); ++k) {
       const int tiles = max(it.tiles[0], it.tiles[1]);
-      for (int j = 0; ok && j < tiles; ++j, n += kQChunks + kVChunks) {
-        const int steps = (min(it.ctx - j * kBK, kBK) + 15) / 16;
-        const uint32_t s0 = (n + kQChunks) % kRing, s1 = (n + kQChunks + 1) % kRing;
+      for (int j = 0; ok && j < tiles; ++j, ++g) {
+        const int inside = min(it.ctx - j * kBK, kBK);  // rows of this V tile that belong to the sequence
+        const int steps = (inside + 15) / 16;
+        const uint32_t s0 = v_chunk(g) % kRing, s1 = (v_chunk(g) + 1) % kRing;
         const uint64_t v0 = sw128_mnmajor_desc(sm + Smem::kKv + s0 * kChunkBytes, kChunkBytes);
         const uint64_t v1 = sw128_mnmajor_desc(sm + Smem::kKv + s1 * kChunkBytes, kChunkBytes);
-        ok = mbar_wait_warp(&bars[Smem::kFull + s0], ((n + kQChunks) / kRing) & 1, p.err) &&
-             mbar_wait_warp(&bars[Smem::kFull + s1], ((n + kQChunks + 1) / kRing) & 1, p.err);
+        ok = mbar_wait_warp(&bars[Smem::kVFull + (g & 1)], (g / 2) & 1, p.err);
+        if (ok && (inside & 15) != 0) {
+          // rows behind the sequence, up to the product's last step of 16, are another's: zeroed,
+          // so that a weight of 0 never meets a non-finite value
+          for (int i = lane; i < (steps * 16 - inside) * 8 * kVChunks; i += 32)
+            *reinterpret_cast<uint4*>(smem + Smem::kKv + ((i & 8) ? s1 : s0) * kChunkBytes + (inside + (i >> 4)) * 128 +
+                                      (i & 7) * 16) = make_uint4(0u, 0u, 0u, 0u);
+          fence_proxy_async_smem();
+          __syncwarp();
+        }
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
           if (!ok || j >= it.tiles[x]) continue;
@@ -385,7 +421,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                mbar_wait_warp(&bars[Smem::kPFull + x], np[x] & 1, p.err);
           if (!ok) continue;
           tc_fence_after();
-          const uint32_t o_tmem = tmem + kTmemO + x * kV, p_tmem = tmem + x * kBK;
+          const uint32_t o_tmem = tmem + kTmemO + x * kV, p_tmem = tmem + kTmemP + x * (kBK / 2);
           if (s1 == s0 + 1) {  // both chunks of V lie together: one product over 128 columns
 #pragma unroll
             for (int k = 0; k < kBK / 16; ++k)
@@ -398,11 +434,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                 umma_tmem_a_elected(o_tmem + 64, p_tmem + k * 8, v1 + k * (2048 >> 4), idesc_half, (j > 0 || k > 0) ? 1u : 0u, elected);
               }
           }
-          if (last_user) {
-            commit_elected(&bars[Smem::kEmpty + s0], elected);
-            commit_elected(&bars[Smem::kEmpty + s1], elected);
-          }
           commit_elected(&bars[Smem::kPvDone + x], elected);
+          if (last_user) commit_elected(&bars[Smem::kVEmpty + (g & 1)], elected);
           ++np[x];
           if (j == 0) ++items[x];
         }
@@ -417,10 +450,10 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int x_tile = warp >> 2;
     const int r = (warp & 3) * 32 + lane;
     const uint32_t lanes = uint32_t((warp & 3) * 32) << 16;
-    const uint32_t s_tmem = tmem + x_tile * kBK + lanes;
+    const uint32_t s_tmem = tmem + lanes;
+    const uint32_t p_tmem = tmem + kTmemP + x_tile * (kBK / 2) + lanes;
     const uint32_t o_tmem = tmem + kTmemO + x_tile * kV + lanes;
-    uint32_t g = 0;  // key tiles done
-    uint32_t n = 0;  // ring chunks passed
+    uint32_t g = 0;  // this tile's key tiles done
     bool ok = true;
     for (int k = 0; ok && walk.get(p, item_of(k), it); ++k) {
       const int tiles = x_tile == 0 ? it.tiles[0] : it.tiles[1];
@@ -446,6 +479,11 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
         for (int c = 0; c < kBK / 32; ++c) {
           tmem_ld_done(x[c]);
+          if (c == 0) {  // (it waits for all of them) the next product may take the scores' place
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&bars[Smem::kSFree]);
+          }
           if (seen < (c + 1) * 32) {
 #pragma unroll
             for (int i = 0; i < 32; ++i)
@@ -458,17 +496,18 @@ __global__ void __launch_bounds__(kThreads, 1)
         // (the scale is positive, so the largest score is the largest scaled one)
         const float top = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * p.scale_log2;
         const float m_new = fmaxf(m, top);
+        // the product of the tile before has used its weights up, and O may be touched
+        if (j > 0 && !mbar_wait_warp(&bars[Smem::kPvDone + x_tile], (g - 1) & 1, p.err)) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
         const bool up = m_new > m + kRescaleLog2;  // also true for the first finite maximum
         if (__any_sync(0xffffffffu, up)) {
           const float alpha = up ? hw_exp2(m - m_new) : 1.f;
           if (up) m = m_new;
           l *= alpha;
           if (j > 0) {
-            if (!mbar_wait_warp(&bars[Smem::kPvDone + x_tile], (g - 1) & 1, p.err)) {
-              ok = false;
-              break;
-            }
-            tc_fence_after();
 #pragma unroll
             for (int c = 0; c < kV / 16; ++c) {
               uint32_t v[16];
@@ -480,7 +519,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
           }
         }
-        // ---- the weights, over the scores they come from ----
+        // ---- the weights ----
         const float m_use = m == -INFINITY ? 0.f : m - kBias<T>;
         const uint64_t scale2 = pack2f(p.scale_log2, p.scale_log2), minus_m = pack2f(-m_use, -m_use);
         uint64_t l2[2] = {0, 0};
@@ -497,7 +536,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             l2[i & 1] = add2(l2[i & 1], pack2f(e0, e1));
             Pair<T>::store(reinterpret_cast<T*>(&pk[i]), e0, e1);
           }
-          tmem_st_16(s_tmem + c * 16, pk);
+          tmem_st_16(p_tmem + c * 16, pk);
         }
         {
           float a, b;
@@ -505,30 +544,12 @@ __global__ void __launch_bounds__(kThreads, 1)
           l += a + b;
         }
         asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
-        const int inside = ctx - j * kBK;  // rows of this V tile that belong to the sequence
-        if (inside < kBK && (inside & 15) != 0) {
-          // rows behind the sequence, up to the product's next step of 16, are another's: zeroed,
-          // so that a weight of 0 never meets a non-finite value
-          const int stop = (inside + 15) & ~15;
-#pragma unroll
-          for (int c = 0; c < kVChunks; ++c) {
-            const uint32_t at = n + kQChunks + c, s = at % kRing;
-            if (!mbar_wait_warp(&bars[Smem::kFull + s], (at / kRing) & 1, p.err)) ok = false;
-            for (int i = r; i < (stop - inside) * 8; i += kBQ)
-              *reinterpret_cast<uint4*>(smem + Smem::kKv + s * kChunkBytes + (inside + (i >> 3)) * 128 + (i & 7) * 16) =
-                  make_uint4(0u, 0u, 0u, 0u);
-          }
-          fence_proxy_async_smem();
-          if (!ok) break;
-        }
-        n += kQChunks + kVChunks;
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&bars[Smem::kPFull + x_tile]);
       }
       if (!ok) break;
       walk.get(p, item_of(k), it);  // (again, rather than hold it through the tiles)
-      n += (max(it.tiles[0], it.tiles[1]) - tiles) * (kQChunks + kVChunks);
       const bool there = r < (x_tile == 0 ? it.rows[0] : it.rows[1]);
       const int64_t tok = it.q_begin + it.q0 + x_tile * kBQ + r;
       T* const orow = static_cast<T*>(p.out) + tok * p.o_tok + int64_t(it.head) * p.o_head;
