@@ -59,7 +59,7 @@ struct Smem {
   static constexpr int kBars = kKv + kRing * kChunkBytes;
   // indexes of the mbarriers: one of each for tile A and B, or for even and odd key tiles
   static constexpr int kQFull = 0, kQEmpty = 2, kKFull = 4, kKEmpty = 6, kVFull = 8, kVEmpty = 10, kSFull = 12,
-                       kPFull = 14, kPvDone = 16, kOFree = 18, kSFree = 20, kMmaDone = 21, kNumBars = 22;
+                       kPFull = 14, kPvDone = 16, kOFree = 18, kSFree = 20, kMmaDone = 21, kKDone = 22, kNumBars = 24;
   static constexpr int kTmemBase = kBars + 8 * kNumBars;
   static constexpr int kBytes = kTmemBase + 16;
 };
@@ -240,6 +240,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(&bars[Smem::kQEmpty + i], 1);
       mbar_init(&bars[Smem::kKFull + i], 1);
       mbar_init(&bars[Smem::kKEmpty + i], 1);
+      mbar_init(&bars[Smem::kKDone + i], 1);
       mbar_init(&bars[Smem::kVFull + i], 1);
       mbar_init(&bars[Smem::kVEmpty + i], 1);
       mbar_init(&bars[Smem::kSFull + i], 1);
@@ -317,6 +318,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       for (int j = 0; ok && j < tiles; ++j) {
         const int row = it.k_begin + j * kBK;
         if (nk >= 3) ok = mbar_wait_warp(&bars[Smem::kVEmpty + ((nk - 3) & 1)], ((nk - 3) / 2) & 1, p.err);
+        if (nk >= 2) ok = ok && mbar_wait_warp(&bars[Smem::kKDone + (nk & 1)], (nk / 2 - 1) & 1, p.err);
         if (!ok) break;
         if (elected) {
           uint64_t* const full = &bars[Smem::kKFull + (nk & 1)];
@@ -371,9 +373,10 @@ __global__ void __launch_bounds__(kThreads, 1)
             for (int k = 0; k < 4; ++k)
               umma_elected(tmem, a0 + c * (kChunkBytes >> 4) + 2 * k, b0 + s * (kChunkBytes >> 4) + 2 * k, idesc,
                            (c | k) ? 1u : 0u, elected);
+            if (last_user && c == 1) commit_elected(&bars[Smem::kKEmpty + (g & 1)], elected);
           }
           commit_elected(&bars[Smem::kSFull + x], elected);
-          if (last_user) commit_elected(&bars[Smem::kKEmpty + (g & 1)], elected);
+          if (last_user) commit_elected(&bars[Smem::kKDone + (g & 1)], elected);
           ++ns;
           if (j + 1 == it.tiles[x]) {
             commit_elected(&bars[Smem::kQEmpty + x], elected);
