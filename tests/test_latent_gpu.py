@@ -284,3 +284,11 @@ def test_expanded_many_short_prompts():
     g = seeded(25)
     lens = torch.randint(0, 40, (150,), generator=g).tolist()
     check_expanded(lens, lens, 3, torch.bfloat16, 26)
+
+
+def test_expanded_items_where_one_row_tile_sees_nothing():
+    """Prompts of both, only the first, and (more queries than keys) only the second tile of rows, and
+    of none, in turn through every CTA."""
+    q_lens = [256, 100, 300, 20, 512, 130] * 20
+    k_lens = [100, 100, 700, 20, 200, 0] * 20
+    check_expanded(q_lens, k_lens, 4, torch.bfloat16, 27)

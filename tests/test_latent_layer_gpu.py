@@ -277,3 +277,30 @@ def test_refusals():
                 dict(out=q), dict(lse=torch.empty(4, 3, device=dev)), dict(k_nope=k.cpu())):
         with pytest.raises((RuntimeError, NotImplementedError)):
             latent_attention_prefill(**(base | bad))
+
+
+def test_a_cache_beyond_32_bit_offsets():
+    """Rows stored into and read from the far end of a 5 GB cache, as from a small one."""
+    dev = cuda_device()
+    g = seeded(49)
+    blocks, page, t, h = 70001, 64, 150, 20
+    big = torch.empty(blocks, page, W, dtype=torch.bfloat16, device=dev)
+    small = torch.zeros(4, page, W, dtype=torch.bfloat16, device=dev)
+    pages = torch.tensor([[blocks - 1, 0, 65536]], dtype=torch.int32)
+    near = torch.tensor([[3, 0, 1]], dtype=torch.int32)
+    x = torch.randn(t, W, generator=g).bfloat16().to(dev)
+    ql, qr = (torch.randn(1, h, n, generator=g).bfloat16().to(dev) for n in (L, R))
+    cs = rope_cos_sin_cache(t, R)
+    pos = torch.arange(t)
+    outs = []
+    for cache, table in ((big, pages), (small, near)):
+        slots = table[0, pos // page].long() * page + pos % page
+        y = x.clone()
+        latent_rope_and_cache(pos.to(dev), None, y[:, :L], y[:, L:], cs, cache, slots.to(dev))
+        out = torch.empty_like(ql)
+        latent_attention(out, ql, qr, cache, torch.tensor([t], dtype=torch.int32, device=dev), table.to(dev), SCALE)
+        outs.append((out, cache[table[0].long().to(dev)].reshape(-1, W)[:t]))
+    torch.cuda.synchronize()
+    assert capi.read_device_error(stream()) == 0
+    for a, b in zip(*outs):
+        assert bits_equal(a.cpu(), b.cpu())

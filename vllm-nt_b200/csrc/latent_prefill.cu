@@ -19,7 +19,7 @@
 // TMEM: S 128 columns, P_A and P_B 64 each, O_A and O_B 128 each.  Items are dealt to and fro over
 // the CTAs, a sequence's last (longest) rows first.
 // Bound: tensor core, 2 * 320 operations a visible (query, key) pair.  A causal prompt of 8192
-// tokens and 32 heads takes 548 us, 1255 TFLOP/s (635 us with an S buffer a tile that also held its
+// tokens and 32 heads takes 550 us, 1250 TFLOP/s (635 us with an S buffer a tile that also held its
 // weights, which kept a tile's next product waiting for P V).
 #include <algorithm>
 
