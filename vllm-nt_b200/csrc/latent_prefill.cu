@@ -61,7 +61,8 @@ struct Smem {
   static constexpr int kQFull = 0, kQEmpty = 2, kKFull = 4, kKEmpty = 6, kVFull = 8, kVEmpty = 10, kSFull = 12,
                        kPFull = 14, kPvDone = 16, kOFree = 18, kSFree = 20, kMmaDone = 21, kKDone = 22, kNumBars = 24;
   static constexpr int kTmemBase = kBars + 8 * kNumBars;
-  static constexpr int kBytes = kTmemBase + 16;
+  static constexpr int kRow = kTmemBase + 16;  // [256 rows] int2: where a softmax thread's output goes
+  static constexpr int kBytes = kRow + kItemRows * 8;
 };
 static_assert(Smem::kBytes <= 227 * 1024, "shared memory");
 
@@ -456,13 +457,16 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t s_tmem = tmem + lanes;
     const uint32_t p_tmem = tmem + kTmemP + x_tile * (kBK / 2) + lanes;
     const uint32_t o_tmem = tmem + kTmemO + x_tile * kV + lanes;
+    int2* const row_of = reinterpret_cast<int2*>(smem + Smem::kRow) + threadIdx.x;
     uint32_t g = 0;  // this tile's key tiles done
     bool ok = true;
     for (int k = 0; ok && walk.get(p, item_of(k), it); ++k) {
       const int tiles = x_tile == 0 ? it.tiles[0] : it.tiles[1];
       // this row sees keys [0, limit)
       const int ctx = it.ctx;
-      const int limit = r >= (x_tile == 0 ? it.rows[0] : it.rows[1]) ? 0
+      const bool there = r < (x_tile == 0 ? it.rows[0] : it.rows[1]);
+      *row_of = make_int2(there ? it.q_begin + it.q0 + x_tile * kBQ + r : -1, it.head);  // (not held through the tiles)
+      const int limit = !there ? 0
                         : p.causal ? min(max(ctx - it.q_len + it.q0 + x_tile * kBQ + r + 1, 0), ctx)
                                    : ctx;
       float m = -INFINITY, l = 0.f;
@@ -552,16 +556,15 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (lane == 0) mbar_arrive(&bars[Smem::kPFull + x_tile]);
       }
       if (!ok) break;
-      walk.get(p, item_of(k), it);  // (again, rather than hold it through the tiles)
-      const bool there = r < (x_tile == 0 ? it.rows[0] : it.rows[1]);
-      const int64_t tok = it.q_begin + it.q0 + x_tile * kBQ + r;
-      T* const orow = static_cast<T*>(p.out) + tok * p.o_tok + int64_t(it.head) * p.o_head;
+      const int2 row = *row_of;
+      T* const orow = static_cast<T*>(p.out) + int64_t(row.x) * p.o_tok + int64_t(row.y) * p.o_head;
+      float* const lse = p.lse == nullptr || row.x < 0 ? nullptr : p.lse + int64_t(row.x) * p.lse_tok + row.y;
       if (tiles == 0) {  // no visible key: zero rows, as for an empty softmax
-        if (there) {
+        if (row.x >= 0) {
 #pragma unroll
           for (int c = 0; c < kV / 8; ++c) reinterpret_cast<uint4*>(orow)[c] = make_uint4(0u, 0u, 0u, 0u);
-          if (p.lse != nullptr) p.lse[tok * p.lse_tok + it.head] = -INFINITY;
         }
+        if (lse != nullptr) *lse = -INFINITY;
         continue;
       }
       // the item's last product is complete: O is final
@@ -574,7 +577,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         uint32_t v[32];
         __syncwarp();
         tmem_ld_32(o_tmem + c * 32, v);
-        if (there) {
+        if (row.x >= 0) {
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             float f[8];
@@ -587,8 +590,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(&bars[Smem::kOFree + x_tile]);  // the next item may overwrite O
-      if (there && p.lse != nullptr)
-        p.lse[tok * p.lse_tok + it.head] = l == 0.f ? -INFINITY : (m - kBias<T> + log2f(l)) * 0.6931471805599453f;
+      if (lse != nullptr) *lse = l == 0.f ? -INFINITY : (m - kBias<T> + log2f(l)) * 0.6931471805599453f;
     }
   }
 

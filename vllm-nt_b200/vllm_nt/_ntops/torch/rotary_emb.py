@@ -58,16 +58,20 @@ def rotary_embedding(
     return query, key
 
 
+def _token_rows(shape, n, head_size):
+    """[tokens, heads * head_size] or [tokens, heads, head_size]: rows that go to the kernel as they are."""
+    return (len(shape) == 2 or (len(shape) == 3 and shape[2] == head_size)) and shape[0] == n
+
+
 def _rotary_either_layout(positions, query, key, head_size, cos_sin_cache, rot, interleaved):
-    # rows of heads [tokens, heads * head_size] and [tokens, heads, head_size] slices go straight in
     if not positions.is_contiguous():
         positions = positions.contiguous()
-    if cos_sin_cache.stride(-1) != 1:
+    if not cos_sin_cache.is_contiguous() and cos_sin_cache.stride(-1) != 1:
         cos_sin_cache = cos_sin_cache.contiguous()
     n = positions.numel()
-    if query.dim() not in (2, 3) or query.shape[0] != n or (query.dim() == 3 and query.shape[2] != head_size):
+    if not _token_rows(query.shape, n, head_size):
         query = _heads(query, n, head_size)
-    if key is not None and (key.dim() not in (2, 3) or key.shape[0] != n or (key.dim() == 3 and key.shape[2] != head_size)):
+    if key is not None and not _token_rows(key.shape, n, head_size):
         key = _heads(key, n, head_size)
     overload("rotary_embedding")(positions, query, key, cos_sin_cache, head_size, rot, interleaved)
 
