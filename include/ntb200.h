@@ -420,7 +420,8 @@ int ntb200_latent_attention(
  * and accumulation, the weights rounded to the input type.  A row that sees no key is zero, its
  * lse -inf; rows behind the last sequence are left as they were; lse may be NULL.
  * max_query_len bounds the query counts (it only sizes the launch).  Sequences that reach
- * outside num_q_tokens or num_k_tokens are skipped and set NTB200_DEVERR_INDEX_RANGE.
+ * outside num_q_tokens or num_k_tokens, or end before they begin, are skipped and set
+ * NTB200_DEVERR_INDEX_RANGE; where cu_seqlens_q falls, those behind are skipped too.
  * dtype BF16 or F16, scale > 0; pointers 16-byte aligned, strides multiples of 8.
  * No workspace.  No counterpart in the reference. */
 int ntb200_latent_attention_prefill(

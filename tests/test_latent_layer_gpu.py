@@ -253,6 +253,25 @@ def test_bad_start_locations_of_prompts_are_reported():
     assert bool((out[10:] == 7.0).all())
 
 
+def test_prompts_behind_a_falling_start_location_are_skipped():
+    """They could overlap the rows before, and their number would be bounded by nothing."""
+    dev = cuda_device()
+    g = seeded(50)
+    q = torch.randn(40, 2, 192, generator=g).half()
+    kv = torch.randn(40, 2, 256, generator=g).half()
+    kr = torch.randn(40, 64, generator=g).half()
+    kvd = kv.to(dev)
+    cu_k = torch.tensor([0, 20, 20, 40] + [40] * 40, dtype=torch.int32, device=dev)
+    cu_q = torch.tensor([0, 20, 5, 25] + [40] * 40, dtype=torch.int32, device=dev)  # the last ones in a later 32
+    out = torch.full((40, 2, 128), 7.0, dtype=torch.float16, device=dev)
+    latent_attention_prefill(out, q.to(dev), kvd[..., :128], kr.to(dev), kvd[..., 128:], cu_q, cu_k, 30, SCALE)
+    torch.cuda.synchronize()
+    assert capi.read_device_error(stream()) == capi.DEVERR_INDEX_RANGE
+    ref, _, tol, _ = reference_expanded(q[:20], kv[..., :128], kr, kv[..., 128:], [0, 20], [0, 20], True)
+    close(out[:20], ref, tol)
+    assert bool((out[20:] == 7.0).all())
+
+
 def test_refusals():
     dev = cuda_device()
     args, out = _decode_case(48, [20, 30], 16)
@@ -304,3 +323,25 @@ def test_a_cache_beyond_32_bit_offsets():
     assert capi.read_device_error(stream()) == 0
     for a, b in zip(*outs):
         assert bits_equal(a.cpu(), b.cpu())
+
+
+def test_calls_without_any_key():
+    """No cached token and no page, and prompts' queries without keys: zero rows, log-sums of -inf."""
+    dev = cuda_device()
+    dt = torch.bfloat16
+    ql, qr = torch.ones(3, 5, L, dtype=dt, device=dev), torch.ones(3, 5, R, dtype=dt, device=dev)
+    lens = torch.zeros(3, dtype=torch.int32, device=dev)
+    for blocks, width in ((0, 0), (2, 0), (2, 4)):
+        out, lse = torch.full_like(ql, 7.0), torch.full((3, 5), 7.0, device=dev)
+        latent_attention(out, ql, qr, torch.full((blocks, 16, W), float("nan"), dtype=dt, device=dev), lens,
+                         torch.full((3, width), -1, dtype=torch.int32, device=dev), SCALE, lse=lse)
+        assert bool((out == 0).all()) and bool((lse == -torch.inf).all())
+    for causal in (True, False):
+        out, lse = torch.full((3, 5, 128), 7.0, dtype=dt, device=dev), torch.full((3, 5), 7.0, device=dev)
+        latent_attention_prefill(out, torch.ones(3, 5, 192, dtype=dt, device=dev), torch.empty(0, 5, 128, dtype=dt, device=dev),
+                                 torch.empty(0, 64, dtype=dt, device=dev), torch.empty(0, 5, 128, dtype=dt, device=dev),
+                                 torch.tensor([0, 3], dtype=torch.int32, device=dev),
+                                 torch.tensor([0, 0], dtype=torch.int32, device=dev), 3, SCALE, causal, lse)
+        assert bool((out == 0).all()) and bool((lse == -torch.inf).all())
+    torch.cuda.synchronize()
+    assert capi.read_device_error(stream()) == 0

@@ -91,6 +91,7 @@ struct Walk {
   int before;  // items of the sequences before them
   int upto;    // this lane's inclusive count within the 32
   int q_begin, q_len, k_begin, ctx;
+  bool broken;  // cu_q fell somewhere before: the sequences behind could overlap, and are left out
 
   __device__ __forceinline__ void load(const PrefillParams& p, int first) {
     const int lane = threadIdx.x & 31;
@@ -102,6 +103,11 @@ struct Walk {
       k_begin = p.cu_k[b];
       q_len = p.cu_q[b + 1] - q_begin;
       ctx = p.cu_k[b + 1] - k_begin;
+    }
+    const unsigned falls = __ballot_sync(0xffffffffu, q_len < 0);
+    if (broken || (falls & ((1u << lane) - 1)) != 0) q_begin = q_len = k_begin = ctx = 0;
+    broken = broken || falls != 0;
+    if (b < p.num_seqs) {
       if (q_begin < 0 || q_len < 0 || q_len > p.num_q - q_begin || k_begin < 0 || ctx < 0 || ctx > p.num_k - k_begin) {
         raise_device_error(p.err, NTB200_DEVERR_INDEX_RANGE);
         q_begin = q_len = k_begin = ctx = 0;
@@ -117,6 +123,7 @@ struct Walk {
 
   __device__ __forceinline__ void begin(const PrefillParams& p) {
     before = 0;
+    broken = false;
     load(p, 0);
   }
 
