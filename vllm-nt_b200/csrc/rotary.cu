@@ -6,9 +6,12 @@
 //
 // rope_cos_sin_cache: row p holds cos(p f_i) and sin(p f_i) of every frequency f_i.  An fp32
 // product p * f_i is off by up to 2^-24 of the angle, 0.008 rad at 128 Ki positions and more
-// beyond: a thread forms its frequency once in fp64, in turns, and walks rows with it in 64-bit
-// fixed point, where an angle is one addition (off by 2^-64 turns a row, on top of the frequency's
-// 2^-53 of the angle); only the part of a turn goes to fp32 (off by at most 2^-26 turns, 2^-23 rad).
+// beyond: a CTA forms its frequencies once in fp64, in turns, and its threads walk rows with them in
+// 64-bit fixed point, where an angle is one addition (off by 2^-64 turns a row, on top of the
+// frequency's 2^-53 of the angle); only what is left beside the nearest quarter turn goes to fp32
+// (off by at most 2^-23 rad).  131075 rows of 32 frequencies in fp32: 7.2 us, 4.66 TB/s of stores
+// (11.7 with the library's sine and cosine, 86 instructions an angle, and a frequency a thread).
+#include <algorithm>
 #include <cmath>
 
 #include "common.cuh"
@@ -111,8 +114,6 @@ int by_table(const RotaryCall& c, int table_dtype, int dtype, bool interleaved) 
 
 // ---- the table ----
 
-constexpr int kMaxThreadRows = 16;
-
 struct TableParams {
   int64_t rows, first, row_stride;
   int half;
@@ -125,15 +126,44 @@ struct TableParams {
   const float* divisors;
 };
 
+// cos and sin, each times `mag`, of two angles in units of 2^-64 turns.  The nearest quarter turn is
+// the top two bits (rounded) and costs nothing; the rest, y with |y| <= pi / 4, takes the Taylor
+// series up to y^9 and y^10, whose next terms are below 2e-9 and 2e-10.  Both angles go through
+// one instruction stream (f32x2).
+__device__ __forceinline__ void cos_sin_2(uint64_t a, uint64_t b, uint64_t mag, float (&c)[2], float (&s)[2]) {
+  constexpr float kStep = float(1.5707963267948966 / 4294967296.0);  // 2^-32 quarter turns in radians
+  const auto both = [](double v) { return pack2f(float(v), float(v)); };
+  const float ya = float(static_cast<int32_t>((a << 2) >> 32)), yb = float(static_cast<int32_t>((b << 2) >> 32));
+  const uint64_t y = mul2(pack2f(ya, yb), pack2f(kStep, kStep));
+  const uint64_t z = mul2(y, y);
+  uint64_t p = fma2(z, both(1.0 / 362880), both(-1.0 / 5040));
+  p = fma2(p, z, both(1.0 / 120));
+  p = fma2(p, z, both(-1.0 / 6));
+  const uint64_t sn = mul2(fma2(mul2(y, z), p, y), mag);
+  p = fma2(z, both(-1.0 / 3628800), both(1.0 / 40320));
+  p = fma2(p, z, both(-1.0 / 720));
+  p = fma2(p, z, both(1.0 / 24));
+  p = fma2(p, z, both(-0.5));
+  const uint64_t cn = mul2(fma2(p, z, both(1.0)), mag);
+  float sv[2], cv[2];
+  unpack2f(sn, sv[0], sv[1]);
+  unpack2f(cn, cv[0], cv[1]);
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const uint32_t q = (static_cast<uint32_t>((i == 0 ? a : b) >> 32) + 0x20000000u) >> 30;
+    const float u = (q & 1) ? cv[i] : sv[i], v = (q & 1) ? sv[i] : cv[i];
+    s[i] = __uint_as_float(__float_as_uint(u) ^ ((q & 2) << 30));
+    c[i] = __uint_as_float(__float_as_uint(v) ^ (((q + 1) & 2) << 30));
+  }
+}
+
 template <typename T>
 __global__ void __launch_bounds__(kThreads) cos_sin_kernel(T* __restrict__ out, const TableParams p) {
   pdl_trigger();
   pdl_wait();
   const int lanes = p.half < kThreads ? p.half : kThreads;  // threads along the frequencies
   const int strip = kThreads / lanes;                       // rows a CTA writes at once
-  if (int(threadIdx.x) >= strip * lanes) return;
-  const int64_t row0 = int64_t(blockIdx.x) * strip * p.thread_rows + threadIdx.x / lanes;
-  for (int i = threadIdx.x % lanes; i < p.half; i += lanes) {
+  const auto frequency = [&](int i) -> uint64_t {
     double f = exp(i * p.log_step) * p.linear;
     if (p.yarn != 0.0) {
       const double share = fmin(fmax((i - p.ramp_lo) * p.ramp_inv, 0.0), 1.0);
@@ -143,31 +173,46 @@ __global__ void __launch_bounds__(kThreads) cos_sin_kernel(T* __restrict__ out, 
     // whole turns count for nothing: the angle of a row is its number times f's part of a turn in
     // units of 2^-64 turns, whose 64-bit product and sums drop the whole turns by themselves
     f *= 0.15915494309189535;
-    const uint64_t unit = static_cast<uint64_t>((f - floor(f)) * 18446744073709551616.0);
+    return static_cast<uint64_t>((f - floor(f)) * 18446744073709551616.0);
+  };
+  __shared__ uint64_t units[kThreads / 2];  // where several threads need a frequency one forms it
+  if (strip > 1) {
+    if (int(threadIdx.x) < lanes) units[threadIdx.x] = frequency(threadIdx.x);
+    __syncthreads();
+  }
+  if (int(threadIdx.x) >= strip * lanes) return;
+  const int64_t row0 = int64_t(blockIdx.x) * strip * p.thread_rows + threadIdx.x / lanes;
+  for (int i = threadIdx.x % lanes; i < p.half; i += lanes) {
+    const uint64_t unit = strip > 1 ? units[i] : frequency(i);
     const uint64_t step = unit * static_cast<uint64_t>(strip);
     uint64_t phase = unit * static_cast<uint64_t>(p.first + row0);
-#pragma unroll 4
-    for (int r = 0; r < p.thread_rows; ++r, phase += step) {
-      const int64_t row = row0 + int64_t(r) * strip;
-      if (row >= p.rows) break;
-      float s, c;
-      sincospif(float(static_cast<int32_t>(phase >> 32)) * 4.656612873077393e-10f, &s, &c);  // half turns
-      T* const o = out + row * p.row_stride;
-      o[i] = Elem<T>::from_f(c * p.magnitude);
-      o[p.half + i] = Elem<T>::from_f(s * p.magnitude);
+    const uint64_t mag = pack2f(p.magnitude, p.magnitude);
+    const int64_t left = p.rows - row0;  // (this thread's rows are strip apart)
+    const int n = int(left <= 0 ? 0 : min((left + strip - 1) / strip, int64_t(p.thread_rows)));
+    const int64_t ahead = strip * p.row_stride;
+    T* o = out + row0 * p.row_stride + i;
+#pragma unroll 2
+    for (int r = 0; r < n; r += 2, phase += 2 * step, o += 2 * ahead) {
+      float s[2], c[2];
+      cos_sin_2(phase, phase + step, mag, c, s);
+      o[0] = Elem<T>::from_f(c[0]);
+      o[p.half] = Elem<T>::from_f(s[0]);
+      if (r + 1 < n) {
+        o[ahead] = Elem<T>::from_f(c[1]);
+        o[ahead + p.half] = Elem<T>::from_f(s[1]);
+      }
     }
   }
 }
 
-// Rows a thread: a frequency costs about as much as 4 of them, so many for a long table (131075 x 64:
-// 11.4 us with 16, 12.9 with 8, 14.1 with 32, whose last wave is part-filled), but a short one is
-// spread over four CTAs an SM first (4096 x 128: 3.3 us with 16, 2.7 with 8).
+// Rows a thread: as many as make one wave of four CTAs an SM (131075 x 64: 7.2 us with four, 8.0 with
+// five, 8.6 with two or three; 8.4 in waves of 16 rows a thread).
 template <typename T>
 int launch_table(void* out, TableParams p, cudaStream_t stream) {
   const int lanes = p.half < kThreads ? p.half : kThreads;
   const int strip = kThreads / lanes;
   const int64_t per = ceil_div(p.rows, int64_t(strip) * num_sms() * 4);
-  p.thread_rows = int(per < 2 ? 2 : per > kMaxThreadRows ? kMaxThreadRows : per);
+  p.thread_rows = int(std::min<int64_t>(std::max<int64_t>(per, 2), 1 << 30));
   const int64_t ctas = ceil_div(p.rows, int64_t(strip) * p.thread_rows);
   if (ctas > 0x7fffffff) return fail(NTB200_ERR_UNSUPPORTED_SHAPE, "rope_cos_sin_cache: too many rows");
   return launch_kernel("rope_cos_sin_cache", cos_sin_kernel<T>, dim3(unsigned(ctas)), dim3(kThreads), 0, stream,
