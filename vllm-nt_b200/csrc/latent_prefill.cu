@@ -24,6 +24,7 @@
 #include <algorithm>
 
 #include "common.cuh"
+#include "latent_ring.cuh"
 #include "tcgen05.cuh"
 
 namespace ntb200 {
@@ -46,12 +47,7 @@ constexpr uint32_t kTmemCols = 512;
 constexpr uint32_t kTmemP = 128;  // S at 0; P_A, P_B at 128, 192
 constexpr uint32_t kTmemO = 256;  // O_A, O_B at 256, 384
 
-// Where in the ring the CTA's g-th key tile lies: its keys in chunks 5 g .. 5 g + 2, its values
-// behind the next tile's keys.  So what a chunk takes the place of is: K_g, of K_g-2's last chunk and V_g-3;
-// V_g, of K_g's first two.
-__device__ __forceinline__ uint32_t k_chunk(uint32_t g) { return g * (kQChunks + kVChunks); }
-__device__ __forceinline__ uint32_t v_chunk(uint32_t g) { return k_chunk(g + 1) + kQChunks; }
-static_assert(kQChunks == 3 && kVChunks == 2 && kRing == 8, "the ring's order");
+static_assert(kQChunks == kRingKeys && kVChunks == kRingValues && kRing == kRingChunks, "the ring's order");
 
 struct Smem {
   static constexpr int kQ = 0;  // [2 tiles][3 chunks]
@@ -170,6 +166,45 @@ __device__ __forceinline__ void tmem_st_16(uint32_t taddr, const uint32_t (&r)[1
       : "memory");
 }
 
+// The ring's operations as the producer's warp makes them (see RingFill).  A wait for key tile g is one for
+// phase g / 2 of barrier g & 1.
+struct RingOps {
+  uint64_t* bars;
+  uint32_t ring;  // its shared-memory address
+  const CUtensorMap *kn_map, *kr_map, *v_map;
+  uint32_t elected;
+  unsigned int* err;
+  int k_head, k_row, v_head, v_row;  // of the next keys and values
+
+  __device__ __forceinline__ bool wait(int bar, uint32_t g) {
+    return mbar_wait_warp(&bars[bar + (g & 1)], (g / 2) & 1, err);
+  }
+  __device__ __forceinline__ bool keys_half_used(uint32_t g) { return wait(Smem::kKEmpty, g); }
+  __device__ __forceinline__ bool keys_used(uint32_t g) { return wait(Smem::kKDone, g); }
+  __device__ __forceinline__ bool values_used(uint32_t g) { return wait(Smem::kVEmpty, g); }
+  __device__ __forceinline__ void load_keys(uint32_t g) {
+    if (elected) {
+      uint64_t* const full = &bars[Smem::kKFull + (g & 1)];
+      mbar_arrive_expect_tx(full, kQChunks * kChunkBytes);
+      for (int c = 0; c < kQChunks; ++c) {
+        const uint32_t dst = ring + (k_chunk(g) + c) % kRing * kChunkBytes;
+        if (c < kNope / 64) tma_load_3d(dst, kn_map, c * 64, k_head, k_row, smem_u32(full));
+        else tma_load_2d(dst, kr_map, 0, k_row, smem_u32(full));
+      }
+    }
+    __syncwarp();
+  }
+  __device__ __forceinline__ void load_values(uint32_t g) {
+    if (elected) {
+      uint64_t* const full = &bars[Smem::kVFull + (g & 1)];
+      mbar_arrive_expect_tx(full, kVChunks * kChunkBytes);
+      for (int c = 0; c < kVChunks; ++c)
+        tma_load_3d(ring + (v_chunk(g) + c) % kRing * kChunkBytes, v_map, c * 64, v_head, v_row, smem_u32(full));
+    }
+    __syncwarp();
+  }
+};
+
 // A CTA's k-th item.  Rounds go over the CTAs to and fro: within a sequence items shrink, and dealt
 // in one direction the first CTA would have the larger item of every round (8192 tokens of 32
 // heads: 14% over the mean, so 2%).
@@ -269,24 +304,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     __syncwarp();
     uint32_t nq[2] = {0, 0};  // Q tiles loaded
-    uint32_t nk = 0, nv = 0;  // key tiles loaded, value tiles loaded (one behind)
-    int v_head = 0, v_row = 0;  // of value tile nv
+    RingOps ops = {bars, sm + Smem::kKv, &kn_map, &kr_map, &v_map, elected, p.err, 0, 0, 0, 0};
+    RingFill fill;
     bool ok = true;
-    auto load_v = [&]() {
-      if (!ok || nv == nk) return;
-      // its keys have been used
-      ok = mbar_wait_warp(&bars[Smem::kKEmpty + (nv & 1)], (nv / 2) & 1, p.err);
-      if (!ok) return;
-      if (elected) {
-        uint64_t* const full = &bars[Smem::kVFull + (nv & 1)];
-        mbar_arrive_expect_tx(full, kVChunks * kChunkBytes);
-        for (int c = 0; c < kVChunks; ++c)
-          tma_load_3d(sm + Smem::kKv + (v_chunk(nv) + c) % kRing * kChunkBytes, &v_map, c * 64, v_head, v_row,
-                      smem_u32(full));
-      }
-      __syncwarp();
-      ++nv;
-    };
     for (int k = 0; ok && walk.get(p, item_of(k), it); ++k) {
       auto load_q = [&](int x) {
         if (!ok || it.tiles[x] == 0) return;
@@ -305,33 +325,21 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int tiles = max(it.tiles[0], it.tiles[1]);
       load_q(0);
       for (int j = 0; ok && j < tiles; ++j) {
-        const int row = it.k_begin + j * kBK;
-        if (nk >= 3) ok = mbar_wait_warp(&bars[Smem::kVEmpty + ((nk - 3) & 1)], ((nk - 3) / 2) & 1, p.err);
-        if (nk >= 2) ok = ok && mbar_wait_warp(&bars[Smem::kKDone + (nk & 1)], (nk / 2 - 1) & 1, p.err);
-        if (!ok) break;
-        if (elected) {
-          uint64_t* const full = &bars[Smem::kKFull + (nk & 1)];
-          mbar_arrive_expect_tx(full, kQChunks * kChunkBytes);
-          for (int c = 0; c < kQChunks; ++c) {
-            const uint32_t dst = sm + Smem::kKv + (k_chunk(nk) + c) % kRing * kChunkBytes;
-            if (c < kNope / 64) tma_load_3d(dst, &kn_map, c * 64, it.head, row, smem_u32(full));
-            else tma_load_2d(dst, &kr_map, 0, row, smem_u32(full));
-          }
-        }
-        __syncwarp();
+        ops.k_head = it.head;
+        ops.k_row = it.k_begin + j * kBK;
+        ok = fill.keys(ops);
         if (j == 0) load_q(1);
-        load_v();  // of the tile before
-        ++nk;
-        v_head = it.head;
-        v_row = row;
+        ok = ok && fill.values_behind(ops);
+        ops.v_head = ops.k_head;
+        ops.v_row = ops.k_row;
       }
     }
-    load_v();
+    ok = ok && fill.last_values(ops);
     // drain the copies that may still be in flight
     for (int x = 0; x < 2; ++x)
       if (nq[x] > 0) mbar_wait_warp(&bars[Smem::kQFull + x], (nq[x] - 1) & 1, p.err);
-    for (uint32_t g = nk > 2 ? nk - 2 : 0; g < nk; ++g) mbar_wait_warp(&bars[Smem::kKFull + (g & 1)], (g / 2) & 1, p.err);
-    for (uint32_t g = nv > 2 ? nv - 2 : 0; g < nv; ++g) mbar_wait_warp(&bars[Smem::kVFull + (g & 1)], (g / 2) & 1, p.err);
+    for (uint32_t g = fill.nk > 2 ? fill.nk - 2 : 0; g < fill.nk; ++g) ops.wait(Smem::kKFull, g);
+    for (uint32_t g = fill.nv > 2 ? fill.nv - 2 : 0; g < fill.nv; ++g) ops.wait(Smem::kVFull, g);
   } else if (warp == kSWarp) {
     // -------------------------- MMA issuer: S = Q K^T --------------------------
     const uint32_t elected = elect_one();
