@@ -391,7 +391,8 @@ int ntb200_latent_rope_and_cache(
  * [num_seqs, max_blocks_per_seq].  max_query_len bounds every query count (longer sequences are
  * skipped), max_seq_len every length (<= 0: max_blocks_per_seq * block_size; it only sizes
  * the launch).  Page ids out of range (their rows read as zeros), lengths beyond the block table
- * (clamped) and inconsistent query_start_loc (skipped) set NTB200_DEVERR_INDEX_RANGE.
+ * (clamped) and inconsistent query_start_loc (skipped) set NTB200_DEVERR_INDEX_RANGE; where
+ * query_start_loc falls, the sequences behind are skipped too.
  * latent_dim 512, rope_dim 64, scale > 0, dtype BF16 or F16, any number of heads; pointers 16-byte
  * aligned, strides multiples of 8.  workspace: ntb200_latent_attention_workspace_size() bytes,
  * 256-byte aligned, of the current device; two calls may share it only in stream order.

@@ -5,9 +5,10 @@ import pytest
 import torch
 
 from _util import bits_equal, cuda_device, seeded, stream
-from test_latent_gpu import SCALE, check_expanded
+from test_latent_gpu import L, R, SCALE, check_expanded, paged, reference
+from test_rotary_layout_gpu import close
 from vllm_nt._ntops import capi
-from vllm_nt._ntops.torch import latent_attention_prefill
+from vllm_nt._ntops.torch import latent_attention, latent_attention_prefill
 
 pytestmark = pytest.mark.gpu
 
@@ -53,3 +54,40 @@ def test_expanded_last_keys_for_one_tile_of_rows_repeat_their_bits():
         assert capi.read_device_error(stream()) == 0
         for out in outs[1:]:
             assert bits_equal(out, outs[0])
+
+
+# ---- start locations that fall ----
+
+FAR = 2_000_000_000
+
+
+@pytest.mark.parametrize("heads", [1, 16, 100])
+@pytest.mark.parametrize("starts,right", [
+    ([0, 5, 3, 8], 1), ([0, 8, 3, 5], 1), ([0, 2, 5, 0, 8], 2), ([3, 1, 4, 8], 0),
+    (list(range(9)) + [2] + list(range(3, 9)), 8), ([0, 5, FAR, -FAR, 3, 8], 1),
+    ([0] * 300 + [4, 6, 5, 8] + [8] * 300, 301),  # past the first sequence of every thread
+], ids=["5-3", "8-3", "5-0", "at once", "all again", "far", "303rd"])
+def test_sequences_behind_a_falling_start_location_are_skipped(starts, right, heads):
+    """The first `right` sequences are right, and the rows that they do not own stay as they were: those
+    behind the fall could own rows of theirs."""
+    dev = cuda_device()
+    g = seeded(63)
+    n = len(starts) - 1
+    lens = [int(x) for x in torch.randint(0, 400 if n < 20 else 40, (n,), generator=g)]
+    cache, table, rows = paged(lens, 16, torch.bfloat16, g)
+    ql = torch.randn(8, heads, L, generator=g).bfloat16()
+    qr = torch.randn(8, heads, R, generator=g).bfloat16()
+    out = torch.full((8, heads, L), 7.0, dtype=torch.bfloat16, device=dev)
+    lse = torch.full((8, heads), 7.0, device=dev)
+    latent_attention(out, ql.to(dev), qr.to(dev), cache.to(dev), torch.tensor(lens, dtype=torch.int32, device=dev),
+                     table.to(dev), SCALE, query_start_loc=torch.tensor(starts, dtype=torch.int32, device=dev), lse=lse)
+    torch.cuda.synchronize()
+    assert capi.read_device_error(stream()) == capi.DEVERR_INDEX_RANGE
+    own = starts[right] if right else 0
+    assert bool((out[own:] == 7.0).all()) and bool((lse[own:] == 7.0).all())
+    if own:
+        ref, ref_lse, tol, lse_tol = reference(ql[:own], qr[:own], rows[:right], starts[: right + 1], SCALE)
+        close(out[:own], ref, tol)
+        seen = ref_lse > -torch.inf
+        assert torch.equal(lse[:own].cpu() > -torch.inf, seen)
+        close(lse[:own].cpu()[seen], ref_lse[seen], lse_tol[seen])

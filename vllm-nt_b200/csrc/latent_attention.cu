@@ -106,12 +106,15 @@ struct Seq {
   int q_begin, q_len, ctx, groups;
 };
 
-// One sequence's lengths; inconsistent metadata is reported and leaves it without groups.
-__device__ __forceinline__ Seq sequence(const LatentParams& p, int b) {
+// One sequence's lengths; inconsistent metadata is reported and leaves it without groups.  `fall`
+// is lowered to the sequence where the start locations fall.
+__device__ __forceinline__ Seq sequence(const LatentParams& p, int b, int* fall = nullptr) {
   Seq s;
   if (p.query_start_loc != nullptr) {
     s.q_begin = p.query_start_loc[b];
-    s.q_len = p.query_start_loc[b + 1] - s.q_begin;
+    const int end = p.query_start_loc[b + 1];
+    s.q_len = end < s.q_begin ? -1 : end - max(s.q_begin, 0);
+    if (fall != nullptr && end < s.q_begin) *fall = min(*fall, b);
   } else {
     s.q_begin = b * p.uniform_q;
     s.q_len = p.uniform_q;
@@ -338,19 +341,32 @@ __global__ void __launch_bounds__(kThreads, 1)
   pdl_wait();  // queries, cache and metadata come from the kernels before
 
   // ---- this CTA's run of its team's tiles ----
-  Seq own = {0, 0, 0, 0};  // this thread's first sequence
-  int64_t mine = 0;
-  if (threadIdx.x < p.num_seqs) {
-    own = sequence(p, threadIdx.x);
-    mine = team_tiles(p, own, team);
-  }
-  const int64_t own_tiles = mine;
-  for (int b = threadIdx.x + kThreads; b < p.num_seqs; b += kThreads) mine += team_tiles(p, sequence(p, b), team);
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
-  if (lane == 0) scan[warp] = mine;
   if (threadIdx.x == 0) p.desc[int64_t(blockIdx.x) * 2] = make_int4(0, 0, 0, 0);  // ends no cut item yet
-  __syncthreads();
+  Seq own;                    // this thread's first sequence
+  int64_t own_tiles;
+  int seqs = p.num_seqs;      // those that count
+  for (;;) {
+    own = {0, 0, 0, 0};
+    int64_t mine = 0;
+    int fall = seqs;
+    if (int(threadIdx.x) < seqs) {
+      own = sequence(p, threadIdx.x, &fall);
+      mine = team_tiles(p, own, team);
+    }
+    own_tiles = mine;
+    for (int b = threadIdx.x + kThreads; b < seqs; b += kThreads) mine += team_tiles(p, sequence(p, b, &fall), team);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
+    if (lane == 0) scan[warp] = mine;
+    if (!__syncthreads_or(fall < seqs)) break;
+    // Start locations that fall: the sequences behind could own rows of those before, and two CTAs would
+    // write them.  Those up to the first fall are counted again, the others left out.
+    if (threadIdx.x == 0) start[0] = seqs;
+    __syncthreads();
+    atomicMin(&start[0], fall);
+    __syncthreads();
+    seqs = start[0];
+  }
   int64_t total = 0;
 #pragma unroll
   for (int w = 0; w < kThreads / 32; ++w) total += scan[w];
@@ -361,13 +377,13 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int64_t count = min(per, total - begin);
   __syncthreads();
   int64_t carry = 0;
-  for (int base = 0; base < p.num_seqs && carry <= begin; base += kThreads) {
+  for (int base = 0; base < seqs && carry <= begin; base += kThreads) {
     const int b = base + threadIdx.x;
     Seq sq = own;
     int64_t c = own_tiles;
     if (base > 0) {
       c = 0;
-      if (b < p.num_seqs) {
+      if (b < seqs) {
         sq = sequence(p, b);
         c = team_tiles(p, sq, team);
       }
