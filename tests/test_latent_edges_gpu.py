@@ -5,7 +5,7 @@ import pytest
 import torch
 
 from _util import bits_equal, cuda_device, seeded, stream
-from test_latent_gpu import L, R, SCALE, check_expanded, paged, reference
+from test_latent_gpu import L, R, SCALE, check_expanded, paged, reference, reference_expanded
 from test_rotary_layout_gpu import close
 from vllm_nt._ntops import capi
 from vllm_nt._ntops.torch import latent_attention, latent_attention_prefill
@@ -91,3 +91,28 @@ def test_sequences_behind_a_falling_start_location_are_skipped(starts, right, he
         seen = ref_lse > -torch.inf
         assert torch.equal(lse[:own].cpu() > -torch.inf, seen)
         close(lse[:own].cpu()[seen], ref_lse[seen], lse_tol[seen])
+
+
+@pytest.mark.parametrize("cu_q,right", [
+    ([0, 20, FAR, -FAR, 5, 30], 1), ([0, 20, FAR, -FAR, 0, 20], 1), ([0, 7, 20, 19, 40], 2),
+    ([0] * 40 + [20, FAR, -FAR] + [5, 30] * 20, 40),  # (in a later 32)
+], ids=["far", "far, the same", "by one", "42nd"])
+def test_prompts_behind_a_fall_between_far_locations_are_skipped(cu_q, right):
+    """The difference of the far locations is positive in 32 bits."""
+    dev = cuda_device()
+    g = seeded(64)
+    n, own = len(cu_q) - 1, cu_q[right]
+    cu_k = list(cu_q[: right + 1]) + [own] * (n - right)
+    q = torch.randn(40, 2, 192, generator=g).half()
+    kv = torch.randn(40, 2, 256, generator=g).half()
+    kr = torch.randn(40, 64, generator=g).half()
+    kvd = kv.to(dev)
+    out = torch.full((40, 2, 128), 7.0, dtype=torch.float16, device=dev)
+    latent_attention_prefill(out, q.to(dev), kvd[..., :128], kr.to(dev), kvd[..., 128:],
+                             torch.tensor(cu_q, dtype=torch.int32, device=dev),
+                             torch.tensor(cu_k, dtype=torch.int32, device=dev), 30, SCALE)
+    torch.cuda.synchronize()
+    assert capi.read_device_error(stream()) == capi.DEVERR_INDEX_RANGE
+    ref, _, tol, _ = reference_expanded(q[:own], kv[..., :128], kr, kv[..., 128:], cu_q[: right + 1], cu_k[: right + 1], True)
+    close(out[:own], ref, tol)
+    assert bool((out[own:] == 7.0).all())

@@ -94,21 +94,24 @@ struct Walk {
     const int b = first + lane;
     base = first;
     q_begin = q_len = k_begin = ctx = 0;
+    bool fall = false;
     if (b < p.num_seqs) {
       q_begin = p.cu_q[b];
       k_begin = p.cu_k[b];
-      q_len = p.cu_q[b + 1] - q_begin;
-      ctx = p.cu_k[b + 1] - k_begin;
-    }
-    const unsigned falls = __ballot_sync(0xffffffffu, q_len < 0);
-    if (broken || (falls & ((1u << lane) - 1)) != 0) q_begin = q_len = k_begin = ctx = 0;
-    broken = broken || falls != 0;
-    if (b < p.num_seqs) {
-      if (q_begin < 0 || q_len < 0 || q_len > p.num_q - q_begin || k_begin < 0 || ctx < 0 || ctx > p.num_k - k_begin) {
+      const int q_end = p.cu_q[b + 1], k_end = p.cu_k[b + 1];
+      fall = q_end < q_begin;
+      // (compared, not subtracted: the difference of far locations wraps)
+      if (q_begin < 0 || fall || q_end > p.num_q || k_begin < 0 || k_end < k_begin || k_end > p.num_k) {
         raise_device_error(p.err, NTB200_DEVERR_INDEX_RANGE);
-        q_begin = q_len = k_begin = ctx = 0;
+        q_begin = k_begin = 0;
+      } else {
+        q_len = q_end - q_begin;
+        ctx = k_end - k_begin;
       }
     }
+    const unsigned falls = __ballot_sync(0xffffffffu, fall);
+    if (broken || (falls & ((1u << lane) - 1)) != 0) q_begin = q_len = k_begin = ctx = 0;
+    broken = broken || falls != 0;
     upto = (q_len + kItemRows - 1) / kItemRows * p.num_heads;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
