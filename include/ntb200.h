@@ -341,7 +341,8 @@ int ntb200_rotary_embedding(const void* positions, int positions_dtype, void* qu
  *   NTB200_ROPE_YARN    f_i = g_i / factor * w_i + g_i * (1 - w_i), w_i a ramp from 0 to 1 over
  *                       i between the frequencies that make beta_fast and beta_slow turns over
  *                       original_max_position positions (rounded outwards to whole i)
- * each divided by freq_divisors[i] where given (fp32 [d/2], device memory).  Frequencies are
+ * each divided by freq_divisors[i] where given (fp32 [d/2], device memory; where the quotient is
+ * infinite or NaN, as for a divisor of 0, cos and sin are NaN).  Frequencies are
  * formed in fp64 and angles in 64-bit fixed-point turns.  dtype F32, BF16 or F16; original_max_position,
  * beta_fast and beta_slow are read for YARN only.  Replaces the host-side table of
  * vLLM's RotaryEmbedding._compute_cos_sin_cache; the reference gathers from that one. */

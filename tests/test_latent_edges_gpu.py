@@ -1,14 +1,20 @@
 """Latent attention and rotary positions where the other files do not reach: the ends of a CTA's work,
 inconsistent start locations, batches and tables of the sizes that take other paths."""
 
+import math
+
 import pytest
 import torch
 
 from _util import bits_equal, cuda_device, seeded, stream
 from test_latent_gpu import L, R, SCALE, check_expanded, paged, reference, reference_expanded
-from test_rotary_layout_gpu import close
+from test_rotary_layout_gpu import U, close
 from vllm_nt._ntops import capi
-from vllm_nt._ntops.torch import latent_attention, latent_attention_prefill
+from vllm_nt._ntops.torch import (
+    latent_attention,
+    latent_attention_prefill,
+    rope_cos_sin_cache,
+)
 
 pytestmark = pytest.mark.gpu
 
@@ -116,3 +122,39 @@ def test_prompts_behind_a_fall_between_far_locations_are_skipped(cu_q, right):
     ref, _, tol, _ = reference_expanded(q[:own], kv[..., :128], kr, kv[..., 128:], cu_q[: right + 1], cu_k[: right + 1], True)
     close(out[:own], ref, tol)
     assert bool((out[own:] == 7.0).all())
+
+
+# ---- the table ----
+
+
+def table_reference(rows, rot, base, first, mag, div=None):
+    """The unscaled table in 64 bits, and its tolerance.
+
+    A frequency comes from ln(base) by a handful of fp64 steps whose errors the exponent
+    multiplies by ln(base): under 7 ln(base) + 13 halves of a last place, and this one's under
+    ln(base) + 4.  The rest beside a quarter turn goes to fp32 with three roundings of at most
+    pi / 4, under 2^-23; the series' steps are off by under 2^-23 of 1.  Then the magnitude's product and
+    the rounding to the type."""
+    f = base ** (-torch.arange(0, rot, 2, dtype=torch.float64) / rot)
+    if div is not None:
+        f = f / div.double()
+    a = (first + torch.arange(rows, dtype=torch.float64))[:, None] * f
+    ref = mag * torch.cat((a.cos(), a.sin()), -1)
+    angle = torch.cat((a, a), -1).abs()
+    return ref, lambda u: (mag * (2.0**-22 + (8 * math.log(base) + 17) * 2.0**-53 * angle)
+                           + (u + 2.0**-24) * ref.abs() + 2.0**-25 * (u == U[torch.float16]))
+
+
+@pytest.mark.parametrize("rot", [64, 1026])
+def test_divisors_without_a_frequency(rot):
+    """f / 0 and f / NaN are no frequency: the columns are NaN, as cos and sin of inf and NaN are.
+    f / inf is 0 and -f turns the other way."""
+    dev = cuda_device()
+    div = torch.ones(rot // 2)
+    div[[0, 3, 9, 20, 31]] = torch.tensor([0.0, float("inf"), float("nan"), -2.0, -0.0])
+    got = rope_cos_sin_cache(100, rot, freq_divisors=div.to(dev), magnitude=1.5, device=dev).cpu()
+    ref, tol = table_reference(100, rot, 10000.0, 0, 1.5, div)
+    none = torch.zeros(rot, dtype=torch.bool)
+    none[[i + h for i in (0, 9, 31) for h in (0, rot // 2)]] = True
+    assert bool(ref[:, none].isnan().all()) and bool(got[:, none].isnan().all())
+    close(got[:, ~none], ref[:, ~none], tol(U[torch.float32])[:, ~none])

@@ -163,30 +163,37 @@ __global__ void __launch_bounds__(kThreads) cos_sin_kernel(T* __restrict__ out, 
   pdl_wait();
   const int lanes = p.half < kThreads ? p.half : kThreads;  // threads along the frequencies
   const int strip = kThreads / lanes;                       // rows a CTA writes at once
-  const auto frequency = [&](int i) -> uint64_t {
+  struct Frequency {
+    uint64_t unit;  // its part of a turn in units of 2^-64 turns
+    float mag;      // of its cosines and sines
+  };
+  const auto frequency = [&](int i) -> Frequency {
     double f = exp(i * p.log_step) * p.linear;
     if (p.yarn != 0.0) {
       const double share = fmin(fmax((i - p.ramp_lo) * p.ramp_inv, 0.0), 1.0);
       f = f * p.yarn * share + f * (1.0 - share);
     }
     if (p.divisors != nullptr) f /= double(p.divisors[i]);
-    // whole turns count for nothing: the angle of a row is its number times f's part of a turn in
-    // units of 2^-64 turns, whose 64-bit product and sums drop the whole turns by themselves
+    // whole turns count for nothing: the angle of a row is its number times f's part of a turn, whose
+    // 64-bit product and sums drop the whole turns by themselves
     f *= 0.15915494309189535;
-    return static_cast<uint64_t>((f - floor(f)) * 18446744073709551616.0);
+    // a divisor of 0 or NaN leaves no frequency, and an integer cannot say so: the magnitude does
+    if (!isfinite(f)) return {0, __int_as_float(0x7fffffff)};
+    return {static_cast<uint64_t>((f - floor(f)) * 18446744073709551616.0), p.magnitude};
   };
-  __shared__ uint64_t units[kThreads / 2];  // where several threads need a frequency one forms it
+  __shared__ Frequency shared[kThreads / 2];  // where several threads need a frequency one forms it
   if (strip > 1) {
-    if (int(threadIdx.x) < lanes) units[threadIdx.x] = frequency(threadIdx.x);
+    if (int(threadIdx.x) < lanes) shared[threadIdx.x] = frequency(threadIdx.x);
     __syncthreads();
   }
   if (int(threadIdx.x) >= strip * lanes) return;
   const int64_t row0 = int64_t(blockIdx.x) * strip * p.thread_rows + threadIdx.x / lanes;
   for (int i = threadIdx.x % lanes; i < p.half; i += lanes) {
-    const uint64_t unit = strip > 1 ? units[i] : frequency(i);
+    const Frequency own = strip > 1 ? shared[i] : frequency(i);
+    const uint64_t unit = own.unit;
     const uint64_t step = unit * static_cast<uint64_t>(strip);
     uint64_t phase = unit * static_cast<uint64_t>(p.first + row0);
-    const uint64_t mag = pack2f(p.magnitude, p.magnitude);
+    const uint64_t mag = pack2f(own.mag, own.mag);
     const int64_t left = p.rows - row0;  // (this thread's rows are strip apart)
     const int n = int(left <= 0 ? 0 : min((left + strip - 1) / strip, int64_t(p.thread_rows)));
     const int64_t ahead = strip * p.row_stride;

@@ -99,8 +99,8 @@ def rope_cos_sin_cache(
     ``"ntk"`` raises base to base * factor^(d/(d-2)), ``"yarn"`` divides those that turn less
     than ``beta_slow`` times over ``original_max_position`` positions, keeps those that turn more
     than ``beta_fast`` times and blends between.  ``freq_divisors`` (float32 [d/2]) divide the
-    frequencies one by one.  cos and sin are multiplied by ``magnitude`` (None: 0.1 ln(factor) + 1
-    for yarn with factor > 1, else 1).  ``out`` may be given instead of dtype and device."""
+    frequencies one by one (a divisor of 0 or NaN leaves NaN in its columns).  cos and sin are
+    multiplied by ``magnitude`` (None: 0.1 ln(factor) + 1 for yarn with factor > 1, else 1).  ``out`` may be given instead of dtype and device."""
     if scaling not in _SCALINGS:
         raise ValueError(f"rope_cos_sin_cache: unknown scaling {scaling!r}")
     if scaling == "yarn" and original_max_position is None:
