@@ -2,19 +2,23 @@
 inconsistent start locations, batches and tables of the sizes that take other paths."""
 
 import math
+import threading
 
 import pytest
 import torch
 
 from _util import bits_equal, cuda_device, seeded, stream
-from test_latent_gpu import L, R, SCALE, check_expanded, paged, reference, reference_expanded
-from test_rotary_layout_gpu import U, close
+from test_latent_gpu import L, R, SCALE, W, check_expanded, paged, reference, reference_expanded
+from test_rotary_layout_gpu import U, close, table, turned
 from vllm_nt._ntops import capi
 from vllm_nt._ntops.torch import (
     latent_attention,
     latent_attention_prefill,
+    latent_rope_and_cache,
     rope_cos_sin_cache,
+    rotary_embedding,
 )
+from vllm_nt._ntops.torch._ext import ops
 
 pytestmark = pytest.mark.gpu
 
@@ -145,6 +149,18 @@ def table_reference(rows, rot, base, first, mag, div=None):
                            + (u + 2.0**-24) * ref.abs() + 2.0**-25 * (u == U[torch.float16]))
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("rows,rot,first", [
+    (20011, 64, 7), (131075, 64, (1 << 20) + 3), (30011, 80, 0),  # 5 (an odd number), 28 and 9 rows a thread
+    (1301, 1026, 5),                                              # 3, a frequency a thread
+    (500001, 2, 1 << 22), (3000, 128, (1 << 31) - 1000),
+])
+def test_tables_of_more_rows_than_one_wave_takes_in_pairs(rows, rot, first, dtype):
+    got = rope_cos_sin_cache(rows, rot, 500000.0, magnitude=1.25, first_position=first, dtype=dtype, device=cuda_device())
+    ref, tol = table_reference(rows, rot, 500000.0, first, 1.25)
+    close(got, ref, tol(U[dtype]))
+
+
 @pytest.mark.parametrize("rot", [64, 1026])
 def test_divisors_without_a_frequency(rot):
     """f / 0 and f / NaN are no frequency: the columns are NaN, as cos and sin of inf and NaN are.
@@ -158,3 +174,168 @@ def test_divisors_without_a_frequency(rot):
     none[[i + h for i in (0, 9, 31) for h in (0, rot // 2)]] = True
     assert bool(ref[:, none].isnan().all()) and bool(got[:, none].isnan().all())
     close(got[:, ~none], ref[:, ~none], tol(U[torch.float32])[:, ~none])
+
+
+# ---- rotations of calls that fill the GPU: four vectors a lane ----
+
+
+@pytest.mark.parametrize("interleaved", [True, False])
+@pytest.mark.parametrize("dtype,table_dtype", [(torch.bfloat16, torch.float32), (torch.float16, torch.float32),
+                                               (torch.bfloat16, torch.bfloat16), (torch.float32, torch.float32)])
+@pytest.mark.parametrize("tokens,hq,hk,head,rot", [
+    (1300, 20, 8, 64, 64), (1200, 33, 1, 128, 128),  # as many vectors a head as divide 32
+    (1300, 22, 1, 96, 96), (1250, 3, 8, 80, 48),     # and not
+    (1250, 2, 1, 64, 10), (1190, 9, 8, 24, 6),       # pair by pair
+])
+def test_rotation_of_many_tokens(tokens, hq, hk, head, rot, dtype, table_dtype, interleaved):
+    dev = cuda_device()
+    g = seeded(tokens + rot)
+    q = torch.randn(tokens, hq, head, generator=g).to(dtype)
+    k = torch.randn(tokens, hk, head, generator=g).to(dtype)
+    pos = torch.randint(0, 5000, (tokens,), generator=g)
+    cs = table(5000, rot, table_dtype)
+    qd, kd = q.to(dev), k.to(dev)
+    ops().rotary_embedding(pos.to(dev), qd, kd, cs.to(dev), head, rot, interleaved)
+    torch.cuda.synchronize()
+    assert capi.read_device_error(stream()) == 0
+    close(qd, *turned(q, cs, pos, rot, interleaved))
+    close(kd, *turned(k, cs, pos, rot, interleaved))
+    assert bits_equal(qd[..., rot:].cpu(), q[..., rot:]) and bits_equal(kd[..., rot:].cpu(), k[..., rot:])
+
+
+@pytest.mark.parametrize("interleaved,skew", [(True, 2), (False, 1)])
+def test_rotation_of_many_unaligned_rows(interleaved, skew):
+    dev = cuda_device()
+    g = seeded(65)
+    t, h, d = 1300, 9, 64
+    wide = torch.randn(t, h, d + 6, generator=g).bfloat16()
+    pos = torch.randint(0, 50, (t,), generator=g)
+    cs = table(50, d)
+    wd = wide.to(dev)
+    rotary_embedding(pos.to(dev), wd[..., skew : skew + d], None, d, cs.to(dev), interleaved=interleaved)
+    close(wd[..., skew : skew + d], *turned(wide[..., skew : skew + d], cs, pos, d, interleaved))
+    assert bits_equal(wd[..., :skew].cpu(), wide[..., :skew])
+    assert bits_equal(wd[..., skew + d :].cpu(), wide[..., skew + d :])
+
+
+# ---- offsets beyond 32 bits ----
+
+
+def far_apart(t, dim, stride):
+    """t's values with `stride` elements from one index of `dim` to the next, in memory of their own."""
+    strides = list(t.contiguous().stride())
+    strides[dim] = stride
+    buf = torch.empty(1 + sum((n - 1) * s for n, s in zip(t.shape, strides)), dtype=t.dtype, device=t.device)
+    return buf.as_strided(t.shape, strides).copy_(t)
+
+
+def test_rotations_beyond_32_bit_offsets():
+    dev = cuda_device()
+    g = seeded(66)
+    q = torch.randn(3, 2, 64, generator=g).bfloat16().to(dev)
+    k = torch.randn(3, 1, 64, generator=g).bfloat16().to(dev)
+    pos, cs = torch.tensor([5, 0, 40], device=dev), table(50, 64).to(dev)
+    for interleaved in (True, False):
+        near, far = (q.clone(), k.clone()), (far_apart(q, 0, 1_200_000_000), far_apart(k, 0, 1_200_000_008))
+        for x, y in (near, far):
+            rotary_embedding(pos, x, y, 64, cs, interleaved=interleaved)
+        assert bits_equal(far[0].cpu(), near[0].cpu()) and bits_equal(far[1].cpu(), near[1].cpu())
+        assert not bits_equal(near[0].cpu(), q.cpu())
+
+
+def test_prompts_beyond_32_bit_offsets():
+    """Queries and outputs far apart by token, keys and values by head."""
+    dev = cuda_device()
+    g = seeded(67)
+    t, h = 300, 3
+    q = torch.randn(t, h, 192, generator=g).bfloat16().to(dev)
+    kv = torch.randn(t, h, 256, generator=g).bfloat16().to(dev)
+    kr = torch.randn(t, 64, generator=g).bfloat16().to(dev)
+    cu = torch.tensor([0, 130, t], dtype=torch.int32, device=dev)
+    near = torch.empty(t, h, 128, dtype=torch.bfloat16, device=dev)
+    far = far_apart(torch.zeros_like(near), 0, 8_000_000)
+    latent_attention_prefill(near, q, kv[..., :128], kr, kv[..., 128:], cu, cu, 170, SCALE)
+    wide = far_apart(kv, 1, 1_200_000_000)
+    latent_attention_prefill(far, far_apart(q, 0, 8_000_000), wide[..., :128], kr, wide[..., 128:], cu, cu, 170, SCALE)
+    assert bits_equal(far.cpu(), near.cpu()) and bool((near != 0).any())
+
+
+def test_absorbed_queries_beyond_32_bit_offsets():
+    dev = cuda_device()
+    g = seeded(68)
+    lens, h = [70, 300, 5], 20
+    cache, pages, _ = paged(lens, 16, torch.bfloat16, g)
+    ql, qr = (torch.randn(3, h, n, generator=g).bfloat16().to(dev) for n in (L, R))
+    args = (cache.to(dev), torch.tensor(lens, dtype=torch.int32, device=dev), pages.to(dev), SCALE)
+    near = torch.empty_like(ql)
+    far = far_apart(torch.zeros_like(ql), 1, 120_000_000)
+    latent_attention(near, ql, qr, *args)
+    latent_attention(far, far_apart(ql, 0, 1_200_000_000), far_apart(qr, 0, 1_200_000_000), *args)
+    assert bits_equal(far.cpu(), near.cpu())
+
+
+# ---- calls from two host threads, and compiled ones ----
+
+
+def layer_inputs(seed, t=40, h=6):
+    dev = cuda_device()
+    g = seeded(seed)
+    x, q = torch.randn(t, W, generator=g).bfloat16().to(dev), torch.randn(t, h, 192, generator=g).bfloat16().to(dev)
+    ql = torch.randn(t, h, L, generator=g).bfloat16().to(dev)
+    kv = torch.randn(t, h, 256, generator=g).bfloat16().to(dev)
+    pages = torch.randperm(8, generator=g)[: -(-t // 16)].to(torch.int32)
+    slots = pages[torch.arange(t) // 16].long() * 16 + torch.arange(t) % 16
+    lens, cu = (torch.tensor(v, dtype=torch.int32, device=dev) for v in ([t], [0, t]))
+    return x, q, ql, kv, torch.arange(t, device=dev), slots.to(dev), lens, cu, pages[None].to(dev)
+
+
+def layer(cs, x, q, ql, kv, pos, slots, lens, cu, pages):
+    """A layer's calls on copies of its inputs: what they write."""
+    x, q = x.clone(), q.clone()
+    t, h = q.shape[:2]
+    cache = torch.zeros(8, 16, W, dtype=x.dtype, device=x.device)
+    latent_rope_and_cache(pos, q[..., 128:], x[:, :L], x[:, L:], cs, cache, slots)
+    absorbed, lse = torch.empty_like(ql), torch.empty(t, h, device=x.device)
+    latent_attention(absorbed, ql, q[..., 128:], cache, lens, pages, SCALE, query_start_loc=cu, lse=lse)
+    out = torch.empty(t, h, 128, dtype=x.dtype, device=x.device)
+    latent_attention_prefill(out, q, kv[..., :128], x[:, L:], kv[..., 128:], cu, cu, 40, SCALE)
+    rotary_embedding(pos, ql[..., :64].clone(), None, 64, cs, interleaved=True)
+    return x, q, cache, absorbed, lse, out
+
+
+def test_two_host_threads():
+    """Each on a stream of its own: the bits of calls alone."""
+    dev = cuda_device()
+    cs = rope_cos_sin_cache(64, R, device=dev)
+    inputs = [layer_inputs(s) for s in (71, 72)]
+    want = [[t.cpu() for t in layer(cs, *i)] for i in inputs]
+    torch.cuda.synchronize()
+    got, errors = [None, None], []
+
+    def work(n):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream(dev)):
+                for _ in range(50):
+                    result = layer(cs, *inputs[n])
+                got[n] = [t.cpu() for t in result]
+        except Exception as e:  # noqa: BLE001
+            errors.append(e)
+
+    threads = [threading.Thread(target=work, args=(n,)) for n in (0, 1)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors, errors
+    for a, b in zip(got, want):
+        assert all(bits_equal(x, y) for x, y in zip(a, b))
+
+
+def test_a_compiled_layer():
+    """Traced whole (no graph break) with the registered shapes: the bits of the calls themselves."""
+    cs = rope_cos_sin_cache(64, R, device=cuda_device())
+    inputs = layer_inputs(73)
+    want = layer(cs, *inputs)
+    got = torch.compile(layer, backend="aot_eager", fullgraph=True)(cs, *inputs)
+    torch.cuda.synchronize()
+    assert all(bits_equal(a.cpu(), b.cpu()) for a, b in zip(got, want))
