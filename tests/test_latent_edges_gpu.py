@@ -8,7 +8,7 @@ import pytest
 import torch
 
 from _util import bits_equal, cuda_device, seeded, stream
-from test_latent_gpu import L, R, SCALE, W, check_expanded, paged, reference, reference_expanded
+from test_latent_gpu import L, R, SCALE, W, check_attention, check_expanded, paged, reference, reference_expanded
 from test_rotary_layout_gpu import U, close, table, turned
 from vllm_nt._ntops import capi
 from vllm_nt._ntops.torch import (
@@ -339,3 +339,77 @@ def test_a_compiled_layer():
     got = torch.compile(layer, backend="aot_eager", fullgraph=True)(cs, *inputs)
     torch.cuda.synchronize()
     assert all(bits_equal(a.cpu(), b.cpu()) for a, b in zip(got, want))
+
+
+# ---- what the arguments allow and the other tests do not call ----
+
+
+@pytest.mark.parametrize("heads", [130, 200, 600])  # 3, 4 and 10 groups of heads (more than there are teams)
+def test_more_heads_than_two_groups(heads):
+    check_attention([300, 0, 17, 70], [1, 2, 0, 1], heads, 32, torch.bfloat16, heads)
+
+
+def test_many_short_sequences_of_two_groups():
+    g = seeded(81)
+    lens = torch.randint(0, 60, (300,), generator=g).tolist()
+    check_attention(lens, [1] * 300, 100, 16, torch.bfloat16, 82)
+
+
+@pytest.mark.parametrize("page", [1024, 4096])
+def test_pages_longer_than_their_sequences(page):
+    check_attention([257, 1, 900], [1, 3, 1], 16, page, torch.float16, page)
+
+
+def test_one_long_chunk():
+    check_attention([700], [600], 20, 64, torch.bfloat16, 83)
+
+
+def test_expanded_with_many_heads():
+    check_expanded([40, 1, 130], [40, 300, 130], 300, torch.bfloat16, 84)
+
+
+@pytest.mark.parametrize("heads,lens,q_lens", [(16, [3000, 5], [1, 1]), (128, [900, 700, 1], [1, 1, 1]), (8, [500, 90], [70, 3])])
+def test_bounds_that_only_size_the_launch(heads, lens, q_lens):
+    """Contexts longer than announced, as a captured call meets them when it is replayed later."""
+    dev = cuda_device()
+    g = seeded(heads)
+    cache, pages, rows = paged(lens, 16, torch.bfloat16, g)
+    starts = [0] + torch.tensor(q_lens).cumsum(0).tolist()
+    ql, qr = (torch.randn(starts[-1], heads, n, generator=g).bfloat16() for n in (L, R))
+    ref, ref_lse, tol, lse_tol = reference(ql, qr, rows, starts, SCALE)
+    for bound in (1, 64, max(lens), 10**9):
+        out, lse = torch.empty_like(ql, device=dev), torch.empty(starts[-1], heads, device=dev)
+        latent_attention(out, ql.to(dev), qr.to(dev), cache.to(dev), torch.tensor(lens, dtype=torch.int32, device=dev),
+                         pages.to(dev), SCALE, query_start_loc=torch.tensor(starts, dtype=torch.int32, device=dev),
+                         max_query_len=max(q_lens), max_seq_len=bound, lse=lse)
+        close(out, ref, tol)
+        close(lse, ref_lse, lse_tol)
+    assert capi.read_device_error(stream()) == 0
+
+
+def test_expanded_bound_that_only_sizes_the_launch():
+    dev = cuda_device()
+    g = seeded(85)
+    lens = [300, 0, 700, 5]
+    cu = torch.tensor([0] + torch.tensor(lens).cumsum(0).tolist(), dtype=torch.int32, device=dev)
+    t = sum(lens)
+    q, kv = torch.randn(t, 2, 192, generator=g).half().to(dev), torch.randn(t, 2, 256, generator=g).half().to(dev)
+    kr = torch.randn(t, 64, generator=g).half().to(dev)
+    outs = [torch.empty(t, 2, 128, dtype=torch.float16, device=dev) for _ in range(3)]
+    for out, bound in zip(outs, (1, 700, 10**6)):
+        latent_attention_prefill(out, q, kv[..., :128], kr, kv[..., 128:], cu, cu, bound, SCALE)
+    assert bits_equal(outs[0], outs[1]) and bits_equal(outs[2], outs[1])
+
+
+def test_queries_shared_by_the_heads():
+    """A query broadcast to the heads (a stride of 0) is read as it is."""
+    dev = cuda_device()
+    g = seeded(86)
+    lens, h = [90, 33], 5
+    cache, pages, rows = paged(lens, 16, torch.bfloat16, g)
+    ql, qr = (torch.randn(2, 1, n, generator=g).bfloat16() for n in (L, R))
+    out = torch.empty(2, h, L, dtype=torch.bfloat16, device=dev)
+    latent_attention(out, ql.to(dev).expand(2, h, L), qr.to(dev).expand(2, h, R), cache.to(dev),
+                     torch.tensor(lens, dtype=torch.int32, device=dev), pages.to(dev), SCALE)
+    ref, _, tol, _ = reference(ql.expand(2, h, L), qr.expand(2, h, R), rows, [0, 1, 2], SCALE)
+    close(out, ref, tol)
