@@ -160,15 +160,6 @@ struct Walk {
   }
 };
 
-__device__ __forceinline__ void tmem_st_16(uint32_t taddr, const uint32_t (&r)[16]) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
-      "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr),
-      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
-      "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
-      : "memory");
-}
-
 // The ring's operations as the producer's warp makes them (see RingFill).  A wait for key tile g is one for
 // phase g / 2 of barrier g & 1.
 struct RingOps {
@@ -215,12 +206,6 @@ __device__ __forceinline__ int item_of(int k) {
   return k * int(gridDim.x) + int((k & 1) ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
 }
 
-__device__ __forceinline__ float hw_exp2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-
 // 32 TMEM columns on their way into registers, which are there once tmem_ld_done has named them.
 __device__ __forceinline__ void tmem_ld_32_begin(uint32_t taddr, uint32_t (&r)[32]) {
   asm volatile(
@@ -241,13 +226,6 @@ __device__ __forceinline__ void tmem_ld_done(uint32_t (&r)[32]) {
                  "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]),
                  "+r"(r[30]), "+r"(r[31])::"memory");
 }
-
-// The running maximum is subtracted less kBias: fp16 weights then span 2^7 .. 2^15 at the
-// row's largest score and reach 2^-31 of it before they vanish (bf16 has fp32's range).
-template <typename T>
-constexpr float kBias = 0.f;
-template <>
-constexpr float kBias<__half> = 7.f;
 
 template <typename T>
 __global__ void __launch_bounds__(kThreads, 1)

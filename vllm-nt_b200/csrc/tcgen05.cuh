@@ -107,6 +107,30 @@ __device__ __forceinline__ void tmem_ld_16(uint32_t taddr, uint32_t (&r)[16]) {
   asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 }
 
+__device__ __forceinline__ void tmem_st_16(uint32_t taddr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+      "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
+      "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+
+// the hardware base-2 exponential (ex2.approx; exp2(-inf) = +0)
+__device__ __forceinline__ float hw_exp2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// Where softmax weights are rounded to T against a running maximum that may lag by 2^8, it is
+// subtracted less kBias: fp16 weights then span 2^7 .. 2^15 at the row's largest score and reach
+// 2^-31 of it before they vanish (bf16 has fp32's range).
+template <typename T>
+constexpr float kBias = 0.f;
+template <>
+constexpr float kBias<__half> = 7.f;
+
 // The lane that issues for a converged warp, and instructions that only it issues: descriptors then
 // live in uniform registers.  From a branch on one lane an MMA of M = 128, N = 64 took 52 cycles to
 // issue and its commit 44; issued this way 48, shared memory's 128 bytes a cycle, and none.
