@@ -387,13 +387,16 @@ int ntb200_latent_rope_and_cache(
  * They are the last of its seq_lens[b] cached tokens: query i sees positions up to
  * seq_lens[b] - q_len + i.  A row that sees nothing is zero, its lse -inf; rows behind the last
  * sequence are left as they were.  fp32 softmax and accumulation, the weights rounded to the
- * input type for their product.  lse may be NULL.
+ * input type for their product.  lse may be NULL.  A cached latent that is not finite can reach every
+ * row whose tile of 64 cached tokens holds it, also one that may not see it (0 times NaN); rows of the
+ * cache behind a sequence's length never do.
  * Cache [num_blocks, block_size, 576], block_size a multiple of 16; block_tables int32
  * [num_seqs, max_blocks_per_seq].  max_query_len bounds every query count (longer sequences are
- * skipped), max_seq_len every length (<= 0: max_blocks_per_seq * block_size; it only sizes
- * the launch).  Page ids out of range (their rows read as zeros), lengths beyond the block table
- * (clamped) and inconsistent query_start_loc (skipped) set NTB200_DEVERR_INDEX_RANGE; where
- * query_start_loc falls, the sequences behind are skipped too.
+ * skipped; 0: nothing is done; with query_start_loc a bound above what the batch has costs time:
+ * query rows are grouped for it), max_seq_len every length (<= 0: max_blocks_per_seq *
+ * block_size; it only sizes the launch).  Page ids out of range (their rows read as zeros), lengths
+ * beyond the block table (clamped) and inconsistent query_start_loc (skipped) set
+ * NTB200_DEVERR_INDEX_RANGE; where query_start_loc falls, the sequences behind are skipped too.
  * latent_dim 512, rope_dim 64, scale > 0, dtype BF16 or F16, any number of heads; pointers 16-byte
  * aligned, strides multiples of 8.  workspace: ntb200_latent_attention_workspace_size() bytes,
  * 256-byte aligned, of the current device; two calls may share it only in stream order.
@@ -421,8 +424,10 @@ int ntb200_latent_attention(
  * rows cu_seqlens_k[b] .. cu_seqlens_k[b + 1], aligned to the end of the keys.  fp32 softmax
  * and accumulation, the weights rounded to the input type.  A row that sees no key is zero, its
  * lse -inf; rows behind the last sequence are left as they were; lse may be NULL.
- * max_query_len bounds the query counts (it only sizes the launch).  Sequences that reach
- * outside num_q_tokens or num_k_tokens, or end before they begin, are skipped and set
+ * A value that is not finite can reach every row of its sequence whose tile of 128 keys holds it, also
+ * one that the mask keeps from it (0 times NaN).
+ * max_query_len bounds the query counts (it only sizes the launch; 0: nothing is done).
+ * Sequences that reach outside num_q_tokens or num_k_tokens, or end before they begin, are skipped and set
  * NTB200_DEVERR_INDEX_RANGE; where cu_seqlens_q falls, those behind are skipped too.
  * dtype BF16 or F16, scale > 0; pointers 16-byte aligned, strides multiples of 8.
  * No workspace.  No counterpart in the reference. */

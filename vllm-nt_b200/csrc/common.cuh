@@ -256,9 +256,9 @@ __device__ __forceinline__ bool mbar_wait_warp(uint64_t* bar, uint32_t parity, u
 
 // And for waits on the critical path of a latency-bound kernel: the clock is read every 256 tries
 // only, because a read of %globaltimer takes as long as a miss to DRAM (latent_attention, 32 decodes
-// of 128 heads at 16384 tokens: 228 us so, 232 us with mbar_wait_warp).  Where the tensor core is
+// of 128 heads at 16384 tokens: 228 us so, 233 us with mbar_wait_warp).  Where the tensor core is
 // the limit the tries in between only take power and issue slots from it
-// (latent_attention_prefill, 8192 tokens of 32 heads: 762 us so, 735 us with mbar_wait_warp).
+// (latent_attention_prefill, 8192 tokens of 32 heads: 574 us so, 538 us with mbar_wait_warp).
 __device__ __forceinline__ bool mbar_spin_warp(uint64_t* bar, uint32_t parity, unsigned int* err) {
   bool ok = mbar_try_wait(bar, parity);
   if (!__all_sync(0xffffffffu, ok)) {

@@ -33,7 +33,7 @@
 // Bound: HBM for a few rows (96 ragged contexts up to 8192, 16 heads: 99 us, 4.6 TB/s, a tile every
 // 3470 cycles where its bytes need 3070).  With 64 rows the MMAs' operands take 2560 cycles of
 // shared memory a tile, and the chain S, softmax, P, O^T through a ring of two tiles 3700 (32 contexts
-// of 16384, 128 heads: 228 us).
+// of 16384, 128 heads: 226 us; 251 us where calls follow each other for long, at the power limit's clock).
 #include <algorithm>
 
 #include "common.cuh"

@@ -19,7 +19,9 @@
 // TMEM: S 128 columns, P_A and P_B 64 each, O_A and O_B 128 each.  Items are dealt to and fro over
 // the CTAs, a sequence's last (longest) rows first.
 // Bound: tensor core, 2 * 320 operations a visible (query, key) pair.  A causal prompt of 8192
-// tokens and 32 heads takes 550 us, 1250 TFLOP/s (635 us with an S buffer a tile that also held its
+// tokens and 32 heads takes 540 to 556 us, 1250 TFLOP/s, in a short run at 1.68 GHz, and 640 us, 1080
+// TFLOP/s, where calls follow each other for long: it draws the power limit, which then leaves 1.44 GHz
+// (635 us in a short run with an S buffer a tile that also held its
 // weights, which kept a tile's next product waiting for P V).
 #include <algorithm>
 

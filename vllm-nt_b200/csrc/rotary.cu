@@ -8,8 +8,10 @@
 // product p * f_i is off by up to 2^-24 of the angle, 0.008 rad at 128 Ki positions and more
 // beyond: a CTA forms its frequencies once in fp64, in turns, and its threads walk rows with them in
 // 64-bit fixed point, where an angle is one addition (off by 2^-64 turns a row, on top of the
-// frequency's 2^-53 of the angle); only what is left beside the nearest quarter turn goes to fp32
-// (off by at most 2^-23 rad).  131075 rows of 32 frequencies in fp32: 7.2 us, 4.66 TB/s of stores
+// frequency's error, at most (7 ln(base) + 13) 2^-53 of the angle: ln(base), its product with i, exp, the
+// scaling and 1 / (2 pi) each round, the first ones in an exponent of up to ln(base)); only what is left
+// beside the nearest quarter turn goes to fp32
+// (off by at most 2^-23 rad).  131075 rows of 32 frequencies in fp32: 7.5 us, 4.5 TB/s of stores
 // (11.7 with the library's sine and cosine, 86 instructions an angle, and a frequency a thread).
 #include <algorithm>
 #include <cmath>
@@ -212,7 +214,7 @@ __global__ void __launch_bounds__(kThreads) cos_sin_kernel(T* __restrict__ out, 
   }
 }
 
-// Rows a thread: as many as make one wave of four CTAs an SM (131075 x 64: 7.2 us with four, 8.0 with
+// Rows a thread: as many as make one wave of four CTAs an SM (131075 x 64, measured side by side: 7.2 us with four, 8.0 with
 // five, 8.6 with two or three; 8.4 in waves of 16 rows a thread).
 template <typename T>
 int launch_table(void* out, TableParams p, cudaStream_t stream) {
