@@ -7,14 +7,16 @@ two softmax warpgroups -- are written here as the kernel has them.  All of it be
 "comes before": program order in each role, and from what completes a phase of a barrier to whoever
 waits for it.  Two things have to follow from the graph alone, whatever anything takes:
 
-* a barrier is waited for by parity, so a phase may be announced only when the phase before it is complete,
-  and complete only when all waits for the phase before it are over;
+* a barrier is waited for by parity, so a phase may be announced or waited for only when the phase before
+  it is complete, and complete only when all waits for the phase before it are over;
 * a copy may land in a chunk only when the products that read what was there are complete."""
 
 import subprocess
 from pathlib import Path
 
 import pytest
+
+from _phases import Graph
 
 CSRC = Path(__file__).resolve().parents[1] / "vllm-nt_b200" / "csrc"
 
@@ -66,49 +68,23 @@ def producer(tmp_path_factory):
     return run
 
 
-# Events are tuples: ("done", barrier, phase) completes a phase, ("seen", barrier, phase, ...) is a wait for
-# it that is over, ("set", barrier, phase) announces a copy.  Barriers of two copies are named by what they
-# count (even and odd tiles, or tile A and B): phase n and what comes next on the same barrier is `step` on.
+# Barriers are named by the tiles that they count (the phase after tile g's is tile g + 2's: even and odd
+# tiles), or by tile A and B of the rows.
 
 
-class Graph:
-    def __init__(self):
-        self.before = {}
-
-    def event(self, e, *after):
-        self.before.setdefault(e, set()).update(a for a in after if a is not None)
-        return e
-
-    def ancestors(self):
-        """Every event's ancestors, as a set."""
-        memo, state = {}, {}
-        for root in self.before:
-            stack = [root]
-            while stack:
-                e = stack[-1]
-                if e in memo:
-                    stack.pop()
-                    continue
-                missing = [a for a in self.before.get(e, ()) if a not in memo]
-                if missing and state.get(e) != "open":
-                    state[e] = "open"
-                    stack.extend(missing)
-                    continue
-                assert not missing, f"{e} waits for itself"
-                memo[e] = set().union(*({a} | memo[a] for a in self.before.get(e, ())))
-                stack.pop()
-        return memo
+def step(bar):
+    return 2 if isinstance(bar, str) and bar[0] in "KV" else 1
 
 
 def build(trace, items):
     """The graph of one CTA that works on items of (key tiles of rows A, of rows B)."""
-    g = Graph()
+    g = Graph(step)
     done = lambda bar, n: ("done", bar, n)  # noqa: E731
 
     last = None
     for i, (what, which, n) in enumerate(trace):  # the producer
         if what == "wait":
-            last = g.event(("seen", which, n, "producer"), last, done(which, n))
+            last = g.wait(which, n, "producer", last)
         else:
             last = g.event(("set", which + "Full", n), last)
             g.event(("copy", which, n), last)
@@ -120,12 +96,12 @@ def build(trace, items):
     last, ns, count = None, 0, [0, 0]
     for item, b, n in zip(items, base, tiles):  # S = Q K^T
         for j in range(n):
-            last = g.event(("seen", "KFull", b + j, "S"), last, done("KFull", b + j))
+            last = g.wait("KFull", b + j, "S", last)
             for x in (0, 1):
                 if j >= item[x]:
                     continue
                 if ns > 0:
-                    last = g.event(("seen", "SFree", ns - 1, "S"), last, done("SFree", ns - 1))
+                    last = g.wait("SFree", ns - 1, "S", last)
                 last = g.event(("issue S", ns), last)
                 # a commit completes when everything issued before it has
                 if x == 1 or j >= item[1]:
@@ -138,13 +114,13 @@ def build(trace, items):
     last, count, begun, pv = None, [0, 0], [0, 0], None
     for item, b, n in zip(items, base, tiles):  # O += P V
         for j in range(n):
-            last = g.event(("seen", "VFull", b + j, "PV"), last, done("VFull", b + j))
+            last = g.wait("VFull", b + j, "PV", last)
             for x in (0, 1):
                 if j >= item[x]:
                     continue
                 if j == 0 and begun[x] > 0:
-                    last = g.event(("seen", ("OFree", x), begun[x] - 1, "PV"), last, done(("OFree", x), begun[x] - 1))
-                last = g.event(("seen", ("PFull", x), count[x], "PV"), last, done(("PFull", x), count[x]))
+                    last = g.wait(("OFree", x), begun[x] - 1, "PV", last)
+                last = g.wait(("PFull", x), count[x], "PV", last)
                 pv = g.event(done(("PvDone", x), count[x]), last, pv)
                 if x == 1 or j >= item[1]:
                     g.event(done("VEmpty", b + j), pv)
@@ -154,35 +130,24 @@ def build(trace, items):
         last, idx, begun = None, 0, 0
         for item in items:
             for j in range(item[x]):
-                last = g.event(("seen", ("SFull", x), idx, "softmax"), last, done(("SFull", x), idx))
+                last = g.wait(("SFull", x), idx, "softmax", last)
                 g.event(done("SFree", product[x, idx]), last)
                 if j > 0:
-                    last = g.event(("seen", ("PvDone", x), idx - 1, "softmax"), last, done(("PvDone", x), idx - 1))
+                    last = g.wait(("PvDone", x), idx - 1, "softmax", last)
                 last = g.event(("weights", x, idx), last)
                 g.event(done(("PFull", x), idx), last)
                 idx += 1
             if item[x] > 0:
-                last = g.event(("seen", ("PvDone", x), idx - 1, "softmax"), last, done(("PvDone", x), idx - 1))
+                last = g.wait(("PvDone", x), idx - 1, "softmax", last)
                 g.event(done(("OFree", x), begun), last)
                 begun += 1
     return g
 
 
-def step(bar):
-    return 2 if isinstance(bar, str) and bar[0] in "KV" else 1  # (tile barriers exist for even and odd tiles)
-
-
 def faults(trace, chunks, items):
     g = build(trace, items)
     anc = g.ancestors()
-    found = []
-    for e in anc:
-        if e[0] == "set" and e[2] >= step(e[1]) and ("done", e[1], e[2] - step(e[1])) not in anc[e]:
-            found.append(f"{e[1]} {e[2]} announced while the copy before it may be on its way")
-        if e[0] == "seen":
-            following = ("done", e[1], e[2] + step(e[1]))
-            if following in anc and e not in anc[following]:
-                found.append(f"{e[1]} {e[2]} may be over and gone before {e[3]} has seen it")
+    found = g.faults(anc)
     # (chunk, in the order of their copies) -> what is in it
     inside = {}
     for what, which, n in trace:

@@ -49,7 +49,7 @@ KERNEL_SOURCES = (
     "sampler.cu",
 )
 SHARED_HEADERS = (CSRC / "common.cuh", CSRC / "tcgen05.cuh", CSRC / "rope_math.cuh", CSRC / "rope_layout.cuh",
-                  CSRC / "latent_ring.cuh", INCLUDE / "ntb200.h", Path(__file__).resolve())
+                  CSRC / "latent_ring.cuh", CSRC / "prefill_phases.cuh", INCLUDE / "ntb200.h", Path(__file__).resolve())
 
 NVCC_FLAGS = [
     "-gencode",

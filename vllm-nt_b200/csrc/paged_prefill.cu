@@ -41,6 +41,7 @@
 // cache (vllm_nt/_ntops/torch/kv_cache.py:24-63) and masks from the upper left
 // (attention.py:61-63); here no copy is made and the mask follows vLLM.
 #include "common.cuh"
+#include "prefill_phases.cuh"
 #include "tcgen05.cuh"
 
 namespace ntb200 {
@@ -84,8 +85,7 @@ struct Smem {
   static constexpr int kVEmpty = kVFull + 8 * kStages;
   static constexpr int kSFull = kVEmpty + 8 * kStages;
   static constexpr int kPFull = kSFull + 16;
-  static constexpr int kPEmpty = kPFull + 16;
-  static constexpr int kPvDone = kPEmpty + 8;     // [2]: O += P V done, per S buffer
+  static constexpr int kPvDone = kPFull + 16;      // [2]: O += P V done (product_phase)
   static constexpr int kOFree = kPvDone + 16;
   static constexpr int kMmaDone = kOFree + 8;
   static constexpr int kPair = kMmaDone + 8;       // 4 mbarriers: the two warps of each row quadrant
@@ -256,7 +256,6 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_kernel(
   uint64_t* v_empty = reinterpret_cast<uint64_t*>(smem + Smem::kVEmpty);
   uint64_t* s_full = reinterpret_cast<uint64_t*>(smem + Smem::kSFull);
   uint64_t* p_full = reinterpret_cast<uint64_t*>(smem + Smem::kPFull);
-  uint64_t* p_empty = reinterpret_cast<uint64_t*>(smem + Smem::kPEmpty);
   uint64_t* pv_done = reinterpret_cast<uint64_t*>(smem + Smem::kPvDone);
   uint64_t* o_free = reinterpret_cast<uint64_t*>(smem + Smem::kOFree);
   uint64_t* mma_done = reinterpret_cast<uint64_t*>(smem + Smem::kMmaDone);
@@ -312,7 +311,6 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_kernel(
       mbar_init(&p_full[a], kSoftmaxThreads / 32);  // one arrive per softmax warp
       mbar_init(&pv_done[a], 1);
     }
-    mbar_init(p_empty, 1);
     mbar_init(o_free, kSoftmaxThreads / 32);
     mbar_init(mma_done, 2);  // a commit from each issuer
     for (int q = 0; q < 4; ++q) mbar_init(reinterpret_cast<uint64_t*>(smem + Smem::kPair) + q, 32 * kRowParts);
@@ -328,6 +326,10 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_kernel(
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
+  auto wait_product = [&](uint32_t g) -> bool {
+    const ProductPhase ph = product_phase(g);
+    return mbar_wait(&pv_done[ph.barrier], ph.parity, p.err);
+  };
 
   if (warp == 0 || (warp >= kExtraWarp && warp < kPvWarp)) {
     // ------------------------------ TMA producers ------------------------------
@@ -441,10 +443,10 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_kernel(
         if (!mbar_wait(&q_full[qb], (nq / 2) & 1, p.err)) break;
         for (int j = 0; j < it.n_tiles; ++j, ++g) {
           // S_g = Q K_g^T into S[g & 1]; the buffer holds P_{g-2} until O += P_{g-2} V_{g-2}
-          // has read it (pv_done[s] completes once per product on this buffer)
+          // has read it
           const int s = g & 1;
           if (!mbar_wait(&k_full[s], (g / kStages) & 1, p.err) ||
-              (g >= 2 && !mbar_wait(&pv_done[s], ((g / 2) - 1) & 1, p.err))) {
+              (g >= 2 && !wait_product(g - 2))) {
             ok = false;
             break;
           }
@@ -502,8 +504,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_kernel(
             umma_f16_tmem_a(tmem + kTmemO, a_tmem, bdesc, idesc_o, (j > 0 || kk > 0) ? 1u : 0u);
           }
           umma_commit(&v_empty[s]);
-          umma_commit(&pv_done[s]);
-          umma_commit(p_empty);
+          umma_commit(&pv_done[product_phase(g).barrier]);
         }
         ++nq;
       }
@@ -630,7 +631,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_kernel(
         // O is rescaled only once O += P_{g-1} V_{g-1} is complete (and before P_g is
         // released, so the next product sees the new scale)
         if (j > 0 && any) {
-          if (!mbar_wait(p_empty, (g - 1) & 1, p.err)) {
+          if (!wait_product(g - 1)) {
             ok = false;
             break;
           }
@@ -672,7 +673,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_kernel(
       }
       if (!ok) break;
       // the item's last product is complete: O is final
-      ok = mbar_wait(p_empty, (g - 1) & 1, p.err);
+      ok = wait_product(g - 1);
       float l = 0.f;
       if (ok) {
         float all[kRowParts];
